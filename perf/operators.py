@@ -104,7 +104,8 @@ def work(case):
         return {"bytes": 2 * e * s + 2 * case["cols"] * s, "flops": 8 * e}
     if case["op"] == "policy":
         e = case["rows"] * case["classes"]
-        return {"bytes": 2 * e * BYTES[case["dtype"]] + 24 * case["rows"], "flops": 10 * e}
+        # a padded row is not read: its gradient is zero
+        return {"bytes": ((0.8 if case["padded"] else 1) + 1) * e * BYTES[case["dtype"]] + 24 * case["rows"], "flops": 10 * e}
     if case["op"] == "muon":
         mats = [(s[0], s[1] * s[2] * s[3]) for s in _matrices(case)]
         return {"bytes": 20 * sum(m * n for m, n in mats), "flops": sum(_ns_flops(m, n) for m, n in mats)}
@@ -190,20 +191,21 @@ def _plain_policy(logits, actions, old, adv, ref, mask):
     old, adv, ref = old.double(), adv.double(), None if ref is None else ref.double()
     ratio = torch.exp(logp - old)
     one, two = ratio * adv, ratio.clamp(1 - CLIP, 1 + CLIP) * adv
-    live = torch.ones_like(adv) if mask is None else mask.double()
+    live = torch.ones_like(adv, dtype=torch.bool) if mask is None else mask
     count = live.sum().clamp(min=1)
+    zero = torch.zeros_like(adv)
     obj = -torch.minimum(one, two)
-    slope = torch.where(one <= two, -one, torch.zeros_like(one))
-    kl = torch.zeros_like(obj)
+    slope = torch.where(one <= two, -one, zero)
+    kl = zero
     if ref is not None:
         kl = torch.exp(ref - logp) - (ref - logp) - 1
         slope = slope + BETA * (1 - torch.exp(ref - logp))
     clipped = (one > two).double()
-    stats = torch.stack(((obj * live).sum(), (kl * live).sum(), (clipped * live).sum())) / count
-    slope = (slope * live / count).float()[:, None]
-    grad = e / total * -slope
+    stats = torch.stack([torch.where(live, t, zero).sum() for t in (obj, kl, clipped)]) / count
+    slope = torch.where(live, slope / count, zero).float()[:, None]
+    grad = torch.where(live[:, None], e / total * -slope, 0.0)
     grad.scatter_add_(1, at, slope)
-    return (stats[0] + BETA * stats[1]).float(), logp.float(), stats.float(), grad.to(logits.dtype)
+    return (stats[0] + BETA * stats[1]).float(), torch.where(live, logp, zero).float(), stats.float(), grad.to(logits.dtype)
 
 
 def _plain_newton_schulz(g):
@@ -300,7 +302,9 @@ def exact(case, seed):
         stats = torch.stack([t[rows].sum() / count for t in (-torch.minimum(one, two), kl, (two < one).double())])
         loss = stats[0] + BETA * stats[1]
         (grad,) = torch.autograd.grad(loss, z)
-        return loss.detach(), logp.detach(), stats.detach(), grad
+        lp = torch.zeros_like(adv)
+        lp[rows] = logp.detach()[rows]
+        return loss.detach(), lp, stats.detach(), grad
     if case["op"] == "muon":
         params, bufs = [], []
         for p in state["params"]:
