@@ -34,6 +34,13 @@ enum step_status {
     STEP_ERR_WORKSPACE = -3       /* workspace too small                             */
 };
 
+/* element types of the entry points that take more than fp32 tensors */
+enum step_dtype {
+    STEP_F32 = 0,
+    STEP_BF16 = 1,
+    STEP_F16 = 2
+};
+
 int step_abi_version(void);
 const char* step_last_error(void);
 
@@ -501,6 +508,61 @@ int step_aff_features(const void* gaits, int in_f64, double* feat, int N, int T,
 /* compute_aff_features/normalize_features.py:1-22: out[n,j] = (feat[n,j] - (max_j+min_j)/2) /
  * ((max_j-min_j)/2), 0 where max_j == min_j; min/max over the N rows.  out (N,F) float32 or float64. */
 int step_aff_normalize(const double* feat, void* out, int out_f64, int N, int F, void* stream);
+
+/* --------------------------------------------------------------------- layer norm ----
+ * y = (x - mu) * rstd * w + b over the rows of a contiguous (rows, cols) matrix, mu / rstd the row's mean and
+ * 1 / sqrt(biased variance + eps).  No counterpart in the reference (its norms are BatchNorms, which need the batch's
+ * statistics: classifier_hybrid/net/classifier.py:46).  x, y, dy, dx of type `dtype`; w, b, dw, db (each nullable: 1 / 0 /
+ * not wanted) of type `wdtype`; statistics and sums in fp32.  mean / rstd (rows floats each, nullable in the forward) are what
+ * the backward takes.  dx nullable.  dw / db: per-block partial sums in ws (step_layernorm_bwd_ws_bytes), added in a
+ * fixed order: the same bits on every call.                                                           */
+int step_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
+                       long long rows, int cols, int dtype, int wdtype, float eps, void* stream);
+size_t step_layernorm_bwd_ws_bytes(long long rows, int cols);
+int step_layernorm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd,
+                       void* dx, void* dw, void* db, long long rows, int cols, int dtype, int wdtype,
+                       void* ws, size_t ws_bytes, void* stream);
+
+/* ----------------------------------------------------------------- clipped policy loss ----
+ * Value and gradient of the clipped policy objective with a KL term over rows of logits (the fine-tuning of a
+ * classifier on ratings; no counterpart in the reference, whose losses are CrossEntropy, utils/processor.py:236, and the
+ * CVAE's).  With lp = log_softmax(z)[a], rho = exp(lp - old):
+ *   loss = SUM_live ( -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A) + beta (exp(ref - lp) - (ref - lp) - 1) )
+ *          / max(#live, 1)
+ * logits (rows, classes) contiguous of type `dtype`; actions int64, old_logp / advantages / ref_logp (nullable: no KL term)
+ * fp32, mask bytes (nullable: every row is live), one per row.  loss[1], stats[3] = {policy part, KL, share of clipped rows},
+ * logp[rows] (0 in masked rows) fp32; dlogits (nullable) like logits and at the same place within 16 bytes.  A masked row is
+ * not read.  An action outside [0, classes) of a live row makes the loss and the row's gradient NaN; nothing is read there.
+ * With `upstream` (a device scalar) only dlogits is written, times *upstream; skip_one: nothing is done where *upstream is
+ * exactly 1 (the caller's dlogits already holds that gradient).  ws: step_policy_loss_ws_bytes(rows).            */
+size_t step_policy_loss_ws_bytes(long long rows);
+int step_policy_loss(const void* logits, const long long* actions, const float* old_logp, const float* advantages,
+                     const float* ref_logp, const unsigned char* mask, double clip_low, double clip_high, double beta,
+                     const float* upstream, int skip_one, float* loss, float* stats, float* logp, void* dlogits,
+                     long long rows, int classes, int dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------ orthogonalised updates (Muon) ----
+ * For every matrix of a list: o = the result of `steps` Newton-Schulz steps X <- a X + (b A + c A^2) X, A = X X^T,
+ * (a, b, c) = (3.4445, -4.7750, 2.0315), from X = g / (|g|_F + eps) (on the transpose where m > n).  No counterpart in the
+ * reference, whose optimizers are Adam and SGD (utils/processor.py:240-255).
+ * An item is a stack of `batch` contiguous (m, n) matrices.  `items` is a HOST array, its pointers are device pointers.
+ *   plain form: out <- o, g and out of type `dtype`; momentum and param NULL.
+ *   optimizer's form (fp32): momentum <- mu momentum + g; u = nesterov ? g + mu momentum : momentum takes g's place;
+ *   param <- param (1 - lr decay) - lr scale o.  (momentum NULL: u = g; param NULL: out <- o.)
+ * The tensors of different items must not overlap (g may be shared).  Accuracy: fp64 where min(m, n) <= 64, otherwise three
+ * f16 matrix-core terms per product with fp32 accumulation, held to fp32's error.  Reproducible bit for bit.
+ * ws: step_newton_schulz_ws_bytes (0 and step_last_error() for a bad list); only the shapes are looked at there.      */
+typedef struct step_ns_item {
+    const void* g;
+    void* out;
+    float* momentum;
+    float* param;
+    int batch, m, n;
+    float scale;
+} step_ns_item;
+size_t step_newton_schulz_ws_bytes(const step_ns_item* items, int count);
+int step_newton_schulz(const step_ns_item* items, int count, int dtype, int steps, float eps, float momentum, int nesterov,
+                       float lr, float decay, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,16 @@ I = ctypes.c_int
 F = ctypes.c_float
 Z = ctypes.c_size_t
 DBL = ctypes.c_double
+LL = ctypes.c_longlong
+
+# enum step_dtype
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class NsItem(ctypes.Structure):
+    """step_ns_item: a stack of matrices for step_newton_schulz"""
+    _fields_ = [("g", P), ("out", P), ("momentum", P), ("param", P), ("batch", I), ("m", I), ("n", I), ("scale", F)]
+
 
 # name -> (restype, argtypes); must match include/step_hip.h
 SIGNATURES = {
@@ -97,6 +107,13 @@ SIGNATURES = {
     "step_bn_rows_bwd_apply": (I, [P, P, P, P, P, P, P, I, I, P]),
     "step_softmax_fwd": (I, [P, P, I, I, P]),
     "step_softmax_bwd": (I, [P, P, P, I, I, P]),
+    "step_layernorm_fwd": (I, [P, P, P, P, P, P, LL, I, I, I, F, P]),
+    "step_layernorm_bwd_ws_bytes": (Z, [LL, I]),
+    "step_layernorm_bwd": (I, [P, P, P, P, P, P, P, P, LL, I, I, I, P, Z, P]),
+    "step_policy_loss_ws_bytes": (Z, [LL]),
+    "step_policy_loss": (I, [P, P, P, P, P, P, DBL, DBL, DBL, P, I, P, P, P, P, LL, I, I, P, Z, P]),
+    "step_newton_schulz_ws_bytes": (Z, [P, I]),
+    "step_newton_schulz": (I, [P, I, I, I, F, F, I, F, F, P, Z, P]),
 }
 
 _lib = None

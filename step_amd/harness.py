@@ -11,9 +11,13 @@ What is reproduced, statement by statement:
   best-checkpoint lookup   processor.py:142-148,447-455 (epoch and accuracy parsed back out of the file name)
   loaders                  main.py:78-88 (batch_size, shuffle=True, drop_last=True for BOTH splits)
 
+Beyond it: ``optimizer="Muon"`` (step_amd.optim: orthogonalised updates for the weights of the convolutions, Adam for the rest)
+and ``per_policy`` (an epoch of fine-tuning on rewards with the clipped policy loss).
+
 What is not: logging (torchlight), h5 loading, plots.  The data are tensors already shaped (N, C, T, V, 1)
 (utils/loader.py:65-66); batches are index slices of a resident tensor instead of a DataLoader's workers.
 """
+import copy
 import math
 import os
 import re
@@ -100,6 +104,13 @@ class EpochRunner:
                                              weight_decay=weight_decay)
         elif optimizer == "Adam":
             self.optimizer = torch.optim.Adam(self.model.parameters(), lr=base_lr, weight_decay=weight_decay)
+        elif optimizer == "Muon":
+            from .optim import Muon
+            # the weights of the convolutions are matrices; edge importances (K, V, V), norms and biases are not
+            mats = [p for p in self.model.parameters() if p.dim() == 4]
+            rest = [p for p in self.model.parameters() if p.dim() != 4]
+            self.optimizer = Muon([{"params": mats}, {"params": rest, "matrices": False}], lr=base_lr, nesterov=nesterov,
+                                  weight_decay=weight_decay)
         else:
             raise ValueError(optimizer)
         self.lr = base_lr
@@ -141,6 +152,41 @@ class EpochRunner:
             losses.append(loss.item())
             self.meta["iter"] += 1
         return float(np.mean(losses))
+
+    def _logits(self, model, data):
+        output, _ = model(data.float())
+        return torch.log(output) if getattr(model, "RETURNS_SOFTMAX", False) else output
+
+    def per_policy(self, reward, reference=None, clip=0.2, beta=0.04, inner=2):
+        """One epoch of fine-tuning on rewards: for every batch an emotion is drawn per gait from the model, rated by
+        ``reward(data, drawn, label)`` -> (N,) (ratings by people, or drawn == label), and the model is moved `inner` times
+        along the clipped policy loss of the ratings' deviations from their mean, held near `reference` (default: the
+        model as it is now) by the KL term.  Returns (mean loss, mean reward)."""
+        from .losses import policy_loss
+        if reference is None:
+            reference = copy.deepcopy(self.model)
+        reference.eval()
+        losses, rewards = [], []
+        for data, label in self._batches(self.train_set):
+            self.model.eval()                                       # the distribution that answers
+            with torch.no_grad():
+                logp = torch.log_softmax(self._logits(self.model, data), 1)
+                cum = logp.exp().cumsum(1)
+                u = torch.rand(len(data), 1, generator=self._gen).to(data.device) * cum[:, -1:]
+                drawn = (cum < u).sum(1).clamp(max=logp.shape[1] - 1)
+                old = logp.gather(1, drawn[:, None])[:, 0]
+                ref = torch.log_softmax(self._logits(reference, data), 1).gather(1, drawn[:, None])[:, 0]
+                got = reward(data, drawn, label).float()
+                adv = (got - got.mean()) / (got.std(unbiased=False) + 1e-6)
+            for _ in range(inner):
+                loss, _, _ = policy_loss(self._logits(self.model, data), drawn, old, adv, ref, clip=clip, beta=beta)
+                self.optimizer.zero_grad()
+                loss.backward()
+                self.optimizer.step()
+                losses.append(loss.item())
+            rewards.append(got.mean().item())
+            self.meta["iter"] += inner
+        return float(np.mean(losses)), float(np.mean(rewards))
 
     def per_test(self):
         self.model.eval()

@@ -1,8 +1,13 @@
-"""CVAE training loss on the GPU with the reference's names and argument order:
+"""Training losses on the GPU.
+
+The CVAE's with the reference's names and argument order:
 ``between_frame_loss(gait1, gait2, thres)`` (generator_cvae/utils/losses.py:7-42) and
 ``vae_loss(x_in, x_out, mean, lsig, beta)`` (generator_cvae/utils/processor_stgcn.py:34-40).
 One HIP launch computes the value and every gradient (step_vae_loss); the reference spends
-O(B*T*V*C) scalar mse_loss calls (~16 s per iteration in its logs) on the same number."""
+O(B*T*V*C) scalar mse_loss calls (~16 s per iteration in its logs) on the same number.
+
+``policy_loss``: the clipped policy objective with a KL term over rows of logits, for fine-tuning a model on ratings of its
+answers.  The reference has no counterpart."""
 import torch
 
 from . import _lib
@@ -57,3 +62,98 @@ def between_frame_loss(gait1, gait2, thres=0.01):
 def vae_loss(x_in, x_out, mean, lsig, beta=1.):
     """processor_stgcn.py:34-40: between_frame_loss(x_in, x_out) + beta * KLD"""
     return _VaeLossFn.apply(x_in, x_out, mean, lsig, beta)
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    """The forward leaves the gradient for an upstream gradient of 1 behind (value and gradient take one pass over the
+    logits); the backward hands it out, or computes it again from the logits where the upstream gradient is not 1 - on
+    the device, with one rounding - or where a retained graph asks a second time."""
+
+    @staticmethod
+    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, beta):
+        classes = logits.shape[-1]
+        rows = logits.numel() // classes
+        z = logits.contiguous()
+        if z.data_ptr() % 16:                     # the gradient, which starts at 16 bytes, is written in the same packs
+            z = z.clone()
+        dev = z.device
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        stats = torch.empty(3, dtype=torch.float32, device=dev)
+        logp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+        need = ctx.needs_input_grad[0]
+        grad = torch.empty_like(z) if need else None
+        ctx.mark_non_differentiable(logp, stats)
+        ctx.config = (clip_low, clip_high, beta)
+        if not rows:
+            loss.zero_(), stats.zero_()
+        else:
+            nb = _lib.query("step_policy_loss_ws_bytes", rows)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+            _lib.call("step_policy_loss", z, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, beta, None, 0,
+                      loss, stats, logp, grad, rows, classes, _lib.DTYPES[z.dtype], ws, nb)
+        if need:
+            ctx.save_for_backward(z, actions, old_logp, advantages, ref_logp, mask)
+            ctx.grad = grad
+        return loss, logp, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _logp, _stats):
+        z, actions, old_logp, advantages, ref_logp, mask = ctx.saved_tensors
+        grad, ctx.grad = ctx.grad, None
+        first = grad is not None
+        if not first:
+            grad = torch.empty_like(z)
+        rows = z.numel() // z.shape[-1]
+        if rows:
+            nb = _lib.query("step_policy_loss_ws_bytes", rows)
+            ws = torch.empty(nb, dtype=torch.uint8, device=z.device)
+            _lib.call("step_policy_loss", z, actions, old_logp, advantages, ref_logp, mask, *ctx.config, g.float().contiguous(),
+                      int(first), None, None, None, grad, rows, z.shape[-1], _lib.DTYPES[z.dtype], ws, nb)
+        return (grad,) + (None,) * 8
+
+
+def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None, clip=0.2, beta=0.0):
+    """Clipped policy loss with a KL term: (loss, logp, stats).
+
+    logits (..., classes) float32, bfloat16 or float16; per row, i.e. of shape logits.shape[:-1] or broadcast to it:
+    actions (integers), old_logp (log probability of the action when it was drawn), advantages, ref_logp (the reference
+    model's, for the KL term) and mask (bool; False: the row does not count and is not read).  With
+    logp = log_softmax(logits)[action], rho = exp(logp - old_logp):
+
+        loss = mean over the mask of  -min(rho A, clamp(rho, 1 - low, 1 + high) A) + beta (exp(d) - d - 1),  d = ref_logp - logp
+
+    (0 where the mask leaves nothing); ``clip`` is low = high or the pair (low, high).  The loss is differentiable in the
+    logits alone.  logp (the rows' log probabilities, 0 where masked) and stats = [policy part, KL, share of clipped rows] are
+    fp32 and carry no gradient.  An action outside [0, classes) in a live row makes the loss NaN.  The gradient (of the logits'
+    type, rounded once) is made in the forward already and takes the logits' size in memory until the backward."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise _lib.StepHipError("policy_loss: logits (..., classes) wanted")
+    if logits.dtype not in _lib.DTYPES:
+        raise _lib.StepHipError("policy_loss: float32, bfloat16 or float16 logits wanted, got %s" % logits.dtype)
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    low, high, beta = float(low), float(high), float(beta)
+    if not (0.0 <= low <= 1.0 and high >= 0.0):
+        raise _lib.StepHipError("policy_loss: clip (%r, %r): 0 <= low <= 1 and high >= 0 wanted" % (low, high))
+    lead = logits.shape[:-1]
+
+    def per_row(t, name, kinds, to):
+        if not isinstance(t, torch.Tensor) or t.dtype not in kinds:
+            raise _lib.StepHipError("policy_loss: %s: a tensor of %s wanted, got %s" % (
+                name, " / ".join(str(k)[6:] for k in kinds), getattr(t, "dtype", type(t).__name__)))
+        if t.device != logits.device:
+            raise _lib.StepHipError("policy_loss: %s is on %s, logits on %s" % (name, t.device, logits.device))
+        try:
+            return t.detach().to(to).expand(lead).contiguous()
+        except RuntimeError:
+            raise _lib.StepHipError("policy_loss: %s %s does not fit logits %s" % (name, tuple(t.shape), tuple(logits.shape))) from None
+
+    floats = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
+    actions = per_row(actions, "actions", (torch.int64, torch.int32), torch.int64)
+    old_logp = per_row(old_logp, "old_logp", floats, torch.float32)
+    advantages = per_row(advantages, "advantages", floats, torch.float32)
+    ref_logp = per_row(ref_logp, "ref_logp", floats, torch.float32) if ref_logp is not None else None
+    mask = per_row(mask, "mask", (torch.bool,), torch.bool) if mask is not None else None
+    if not logits.is_cuda:
+        raise _lib.StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % logits.device)
+    return _PolicyLossFn.apply(logits, actions, old_logp, advantages, ref_logp, mask, low, high, beta)

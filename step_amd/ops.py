@@ -797,3 +797,78 @@ class BnRowsFn(torch.autograd.Function):
             return None, None, dx, dg, db
         _lib.call("step_bn_rows_bwd", _f32(dy), x, mean, invstd, weight, int(ctx.training), dx, dg, db, N, G)
         return None, None, dx, dg, db
+
+
+# ----------------------------------------------------------------------- layer norm
+def _dtype_code(t, what):
+    code = _lib.DTYPES.get(t.dtype)
+    if code is None:
+        raise _lib.StepHipError("%s: float32, bfloat16 or float16 wanted, got %s" % (what, t.dtype))
+    return code
+
+
+class LayerNormFn(torch.autograd.Function):
+    """Layer norm over the last axis; saves the rows' mean and 1 / sqrt(variance + eps) for the backward"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        cols = x.shape[-1]
+        xc = x.contiguous()
+        rows = xc.numel() // cols
+        w = weight.contiguous() if weight is not None else None
+        b = bias.contiguous() if bias is not None else None
+        wcode = _lib.DTYPES[w.dtype] if w is not None else _lib.DTYPES[b.dtype] if b is not None else 0
+        y = torch.empty_like(xc)
+        keep = any(ctx.needs_input_grad[:3])
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+        mean, rstd = (stats[0], stats[1]) if keep else (None, None)
+        if rows:
+            _lib.call("step_layernorm_fwd", xc, w, b, y, mean, rstd, rows, cols, _lib.DTYPES[x.dtype], wcode, eps)
+        if keep:
+            ctx.save_for_backward(xc, w, stats)
+            ctx.codes = (_lib.DTYPES[x.dtype], wcode)
+            ctx.wtype = w.dtype if w is not None else b.dtype if b is not None else None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        cols = x.shape[-1]
+        rows = x.numel() // cols
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty(cols, dtype=ctx.wtype, device=x.device) if need_w else None
+        db = torch.empty(cols, dtype=ctx.wtype, device=x.device) if need_b else None
+        if not rows:
+            return dx, dw.zero_() if need_w else None, db.zero_() if need_b else None, None
+        nb = _lib.query("step_layernorm_bwd_ws_bytes", rows, cols) if need_w or need_b else 0
+        ws = _ws(nb, x.device) if nb else None
+        _lib.call("step_layernorm_bwd", dy.contiguous(), x, w, stats[0], stats[1], dx, dw, db, rows, cols, *ctx.codes, ws, nb)
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (any leading axes; biased variance).
+
+    x float32, bfloat16 or float16; weight and bias (cols,) of x's type or float32, either may be None.  Statistics and
+    gradient sums are fp32, every result is rounded once.  Needs no statistics of the batch: a row's result is the same
+    in any batch, on any number of ranks and for a single row."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise _lib.StepHipError("layer_norm: x %s has no last axis to normalise" % (tuple(x.shape),))
+    _dtype_code(x, "layer_norm")
+    cols = x.shape[-1]
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (cols,):
+            raise _lib.StepHipError("layer_norm: %s %s does not fit x %s" % (name, tuple(t.shape), tuple(x.shape)))
+        if t.dtype not in (x.dtype, torch.float32):
+            raise _lib.StepHipError("layer_norm: %s is %s; %s or float32 wanted" % (name, t.dtype, x.dtype))
+        if t.device != x.device:
+            raise _lib.StepHipError("layer_norm: %s is on %s, x on %s" % (name, t.device, x.device))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise _lib.StepHipError("layer_norm: weight is %s, bias %s" % (weight.dtype, bias.dtype))
+    if not x.is_cuda:
+        raise _lib.StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % x.device)
+    return LayerNormFn.apply(x, weight, bias, float(eps))

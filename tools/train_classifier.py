@@ -31,6 +31,9 @@ def main():
     ap.add_argument("--work-dir", default="/tmp/step_amd_train")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--variant", choices=["real_only", "real_and_synth"], default="real_only")
+    ap.add_argument("--optimizer", choices=["Adam", "SGD", "Muon"], default="Adam")
+    ap.add_argument("--policy-epochs", type=int, default=0,
+                    help="epochs of fine-tuning with the clipped policy loss afterwards (reward: the drawn emotion is the label)")
     args = ap.parse_args()
 
     from step_amd import harness
@@ -40,13 +43,15 @@ def main():
     model = mod.Classifier(3, 4, {"strategy": "spatial"})
     train_set, test_set = harness.synthetic_gaits(args.gaits, args.frames, 4, args.seed)
     run = harness.EpochRunner(model, train_set, test_set, args.work_dir, args.num_epoch, args.batch_size,
-                              args.base_lr, args.weight_decay, seed=args.seed, log=lambda s: print(s, flush=True))
+                              args.base_lr, args.weight_decay, optimizer=args.optimizer, seed=args.seed, log=lambda s: print(s, flush=True))
     t0 = time.perf_counter()
     hist = run.train()
     torch.cuda.synchronize()
     dt = time.perf_counter() - t0
     path = run.load_best_model()
     loss, acc = run.per_test()
+    for _ in range(args.policy_epochs):
+        print("policy: loss %.6f, mean reward %.4f" % run.per_policy(lambda data, drawn, label: (drawn == label)), flush=True)
     print(json.dumps({"epochs": len(hist), "seconds": round(dt, 2), "iterations": run.meta["iter"],
                       "sequences_per_s": round(run.meta["iter"] * args.batch_size / dt, 1),
                       "best_checkpoint": os.path.basename(path), "reloaded_top1": acc[1], "reloaded_loss": loss,
