@@ -534,7 +534,8 @@ int step_layernorm_bwd(const void* dy, const void* x, const void* w, const float
  * logp[rows] (0 in masked rows) fp32; dlogits (nullable) like logits and at the same place within 16 bytes.  A masked row is
  * not read.  An action outside [0, classes) of a live row makes the loss and the row's gradient NaN; nothing is read there.
  * With `upstream` (a device scalar) only dlogits is written, times *upstream; skip_one: nothing is done where *upstream is
- * exactly 1 (the caller's dlogits already holds that gradient).  ws: step_policy_loss_ws_bytes(rows).            */
+ * exactly 1 (the caller's dlogits already holds that gradient), and ws is the one that the call without `upstream` left (it
+ * holds the number of live rows).  ws: step_policy_loss_ws_bytes(rows).                                       */
 size_t step_policy_loss_ws_bytes(long long rows);
 int step_policy_loss(const void* logits, const long long* actions, const float* old_logp, const float* advantages,
                      const float* ref_logp, const unsigned char* mask, double clip_low, double clip_high, double beta,

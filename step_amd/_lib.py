@@ -154,7 +154,8 @@ def _ptr(t):
 
 
 def stream(device=None):
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)     # (no Stream object: 0.3 us a launch instead of 2 to 9)
 
 
 def call(name, *args):

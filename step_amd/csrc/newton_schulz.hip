@@ -275,22 +275,21 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const SmallArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- r > 64
-constexpr int TILE = 128, KS = 32;                // output tile, contraction per stage
+constexpr int TN = 128, KS = 32;                  // columns of an output tile, contraction per stage
 constexpr int ROWB = 128;                         // bytes of a row's stage: 32 hi, 32 lo
-constexpr int EP = TILE + 4;                      // pitch of the tile in LDS at the end
+constexpr int EP = TN + 4;                        // pitch of a tile in LDS at the end
 constexpr float SX = 16384.f, SA = 16384.f, SB = 8192.f;   // scales of X, A and q(A): elements under 1.21, 1.47, 3.45
+constexpr int CUS = 256;
+constexpr int NORM_BLOCKS = 1024;
 
 struct Big {
     Io io;
-    int m, n, r, l, R, L;                         // R, L: r and l rounded up to whole tiles
-    int bytes;                                    // of an element
+    int m, n, r, l, R, L, RA;                     // R, L: r and l rounded up to whole tiles; RA: rows that X and A have
     float eps;
     double* part;                                 // [batch][NORM_BLOCKS] sums of squares
     char *x, *xt, *xt2, *a, *b;                   // packed matrices, one after the other for the batch
-    float* slab;                                  // [batch][tiles][splits] partial tiles
-    int splits;
+    float* slab;                                  // shares of split tiles
 };
-constexpr int NORM_BLOCKS = 256;
 
 template <typename T>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const Big p) {
@@ -298,9 +297,23 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const Big p) {
     const size_t e = (size_t)p.m * p.n;
     const Io io = shifted(p.io, e * blockIdx.y, sizeof(T));
     double s = 0.0;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < e; i += (size_t)gridDim.x * 256) {
-        const double v = (double)read_u<T>(io, i, true);
-        s += v * v;
+    constexpr int N = 16 / (int)sizeof(T);
+    if (!io.momentum && ((uintptr_t)io.g & 15) == 0) {
+        const size_t packs = e / N;
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) {
+            const Pack<T, N> q = ((const Pack<T, N>*)io.g)[i];
+#pragma unroll
+            for (int k = 0; k < N; ++k) s += (double)(float)q.v[k] * (double)(float)q.v[k];
+        }
+        if (blockIdx.x == 0 && threadIdx.x < (unsigned)(e - packs * N)) {
+            const double v = (double)(float)((const T*)io.g)[packs * N + threadIdx.x];
+            s += v * v;
+        }
+    } else {
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < e; i += (size_t)gridDim.x * 256) {
+            const double v = (double)read_u<T>(io, i, true);
+            s += v * v;
+        }
     }
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -319,14 +332,22 @@ __device__ __forceinline__ void split8(const float* v, f16x8& hi, f16x8& lo) {
 __device__ __forceinline__ char* packed(char* base, size_t row, int k, int K) {
     return base + (row * (K / KS) + k / KS) * ROWB + (k % KS) * 2;
 }
+__device__ __forceinline__ void put8(char* to, const float* v) {
+    f16x8 hi, lo;
+    split8(v, hi, lo);
+    *(f16x8*)to = hi;
+    *(f16x8*)(to + 64) = lo;
+}
 
-// X_0 scaled and packed, both ways: one 64 x 64 tile a block
+// X_0 scaled and packed, both ways: one 64 x 64 tile a block.  Rows behind R (X has RA) become zero; A's become so too: the
+// products read them, whose results are not written.
 template <typename T>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     __shared__ float sm[64][65];
     __shared__ double red[4];
     const int tid = threadIdx.x, z = blockIdx.z;
-    double s = p.part[(size_t)z * NORM_BLOCKS + tid];
+    double s = 0.0;
+    for (int i = tid; i < NORM_BLOCKS; i += 256) s += p.part[(size_t)z * NORM_BLOCKS + i];
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
@@ -341,298 +362,424 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
         sm[i - i0][k - k0] = v;
     }
     __syncthreads();
-    char* x = p.x + (size_t)z * p.R * p.L * 4;
+    char* x = p.x + (size_t)z * p.RA * p.L * 4;
     char* xt = p.xt + (size_t)z * p.R * p.L * 4;
     for (int u = tid; u < 512; u += 256) {
         float v[8];
-        f16x8 hi, lo;
         const int a = u >> 3, b = (u & 7) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sm[a][b + e];
-        split8(v, hi, lo);
-        char* d = packed(x, i0 + a, k0 + b, p.L);
-        *(f16x8*)d = hi;
-        *(f16x8*)(d + 64) = lo;
+        put8(packed(x, i0 + a, k0 + b, p.L), v);
+        if (i0 >= p.R) {
+            if (k0 + b < p.R) put8(packed(p.a + (size_t)z * p.RA * p.R * 4, i0 + a, k0 + b, p.R), v);
+            continue;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sm[b + e][a];
-        split8(v, hi, lo);
-        d = packed(xt, k0 + a, i0 + b, p.R);
-        *(f16x8*)d = hi;
-        *(f16x8*)(d + 64) = lo;
+        put8(packed(xt, k0 + a, i0 + b, p.R), v);
     }
 }
 
-// a wave's 64 x 64 share of a tile: the products of the hi parts, and the two small terms in sums of their own, so that the
-// large sum is rounded once per product and not three times
+// A wave's 32 MT x 64 share of a tile: the products of the hi parts, and the two small terms in sums of their own, so that the
+// large sum is rounded once per product and not three times.
+template <int MT>
 struct Acc {
-    f32x16 v[2][2], w[2][2];
+    f32x16 v[MT][2], w[MT][2];
 };
-
-// acc += rows [i0, i0 + 128) of A times rows [j0, j0 + 128) of B over the stages [s0, s1): operands packed alike, K along
-// both.  128 rows of a stage are 16 KiB, two stages in LDS; a row's eight 16-byte pieces lie in the order piece ^ (row & 7),
-// so that eight neighbouring rows are read from different banks.
-__device__ __forceinline__ void main_loop(Acc& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, q = lane >> 5;
-    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
-    const size_t pitch = (size_t)(K / KS) * ROWB;
-    // a wave's load: 8 rows x 128 bytes; lane -> row lane / 8, piece (lane % 8) ^ row
-    const int lrow = lane >> 3, piece = (lane & 7) ^ lrow;
-    const char* src = (wave < 2 ? A + (size_t)(i0 + (wave & 1) * 64 + lrow) * pitch : B + (size_t)(j0 + (wave & 1) * 64 + lrow) * pitch) + piece * 16;
-    auto issue = [&](int s, int buf) {
+template <int MT>
+struct Frag {
+    f16x8 ah[MT], al[MT], bh[2], bl[2];
+};
+template <int MT>
+__device__ __forceinline__ void multiply(Acc<MT>& acc, const Frag<MT>& f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (size_t)s * ROWB + i * 8 * pitch),
-                                             (__attribute__((address_space(3))) void*)(lds + buf * 32768 + wave * 8192 + i * 1024), 16, 0, 0);
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[a], f.bh[b], acc.w[a][b], 0, 0, 0);
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc.v[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bh[b], acc.v[a][b], 0, 0, 0);
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bl[b], acc.w[a][b], 0, 0, 0);
+}
+
+// acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 128) of B over the stages [s0, s1): operands packed alike, K along both.
+// A stage lies in LDS as rows of 128 bytes whose eight 16-byte pieces are in the order piece ^ order(row): 16 neighbouring rows
+// are read from different banks (64 banks hold two rows).  Three stages in LDS, copied there directly, two of them in flight.  A wave reads the
+// operands of the next half stage before it multiplies the present one; one barrier a stage, in the middle: before it a
+// wave has its reads of the stage behind it and its copies of the next one, after it the stage's place is filled again.
+// The tile is what LDS reads allow: 192 rows read per 128 x 64 x 3 products keep the matrix cores ahead of LDS (94 of 128
+// bytes a cycle); 64 x 64 a wave needs 125.
+template <int MT>
+__device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
+    constexpr int TM = 64 * MT, STAGE = (TM + TN) * ROWB, NA = TM / 32, NL = NA + 4;      // copies of a wave: NA + 4 of 8 rows
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, q = lane >> 5;
+    const size_t pitch = (size_t)(K / KS) * ROWB;
+    const int lrow = lane >> 3, piece = (lane & 7) ^ lrow, order = (l31 & 7) ^ ((l31 >> 3) & 1);
+    // a copy's address: the panel's descriptor, this lane's place in it, and a scalar offset
+    const __amdgpu_buffer_rsrc_t pa = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (size_t)i0 * pitch), 0, 0xffffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t pb = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (size_t)j0 * pitch), 0, 0xffffffff, 0x00020000);
+    const unsigned va = (unsigned)((wave * (TM / 4) + lrow) * pitch), vb = (unsigned)((wave * 32 + lrow) * pitch);
+    const unsigned at8[2] = {piece * 16u, (piece ^ 1) * 16u};                // rows 0 .. 7 and 8 .. 15 of each 16
+    const unsigned row8 = (unsigned)(8 * pitch);
+    char* da = lds + wave * (TM / 4) * ROWB;
+    char* db = lds + TM * ROWB + wave * 32 * ROWB;
+    auto copy = [](__amdgpu_buffer_rsrc_t from, unsigned lane_at, unsigned at, char* to) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, (int)lane_at, (int)at, 0, 0);
+    };
+    auto issue = [&](int s, int buf) {
+        const unsigned at = (unsigned)(s < s1 ? s : s1 - 1) * ROWB;          // behind the end: any stage, never used
+#pragma unroll
+        for (int i = 0; i < NA; ++i) copy(pa, va + at8[i & 1], at + i * row8, da + buf * STAGE + i * 1024);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) copy(pb, vb + at8[i & 1], at + i * row8, db + buf * STAGE + i * 1024);
+    };
+    const char* ra = lds + ((wave >> 1) * (TM / 2) + l31) * ROWB;
+    const char* rb = lds + (TM + (wave & 1) * 64 + l31) * ROWB;
+    auto read = [&](Frag<MT>& f, int buf, int kk) {
+        const int hi = buf * STAGE + (((kk * 2 + q) ^ order) * 16), lo = buf * STAGE + (((4 + kk * 2 + q) ^ order) * 16);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            f.al[t] = *(const f16x8*)(ra + lo + t * 32 * ROWB);
+            f.ah[t] = *(const f16x8*)(ra + hi + t * 32 * ROWB);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f.bh[t] = *(const f16x8*)(rb + hi + t * 32 * ROWB);
+            f.bl[t] = *(const f16x8*)(rb + lo + t * 32 * ROWB);
+        }
     };
     issue(s0, 0);
+    issue(s0 + 1, 1);
+    issue(s0 + 2, 2);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+    __builtin_amdgcn_s_barrier();
+    Frag<MT> f0, f1;
+    read(f0, 0, 0);
+    int buf = 0;
     for (int s = s0; s < s1; ++s) {
-        const int buf = (s - s0) & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the stage has arrived
-        __syncthreads();                          // everybody's has, and the other stage is read
-        if (s + 1 < s1) issue(s + 1, buf ^ 1);
-        const char* la = lds + buf * 32768;
-        const char* lb = la + 16384;
+        const int next = buf == 2 ? 0 : buf + 1;
+        __builtin_amdgcn_s_waitcnt(0xc07f);       // lgkmcnt(0): f0, read half a stage ago.  (The builtin, which the compiler counts
+        __builtin_amdgcn_sched_barrier(0);        // too: else it waits for f1 as well before f0 is used.)
+        read(f1, buf, 1);
+        multiply(acc, f0);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            f16x8 ah[2], al[2], bh[2], bl[2];
-            const int ph = kk * 2 + q, pl = 4 + ph;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int ra = wi + 32 * t + l31, rb = wj + 32 * t + l31;
-                ah[t] = *(const f16x8*)(la + ra * ROWB + ((ph ^ (ra & 7)) * 16));
-                al[t] = *(const f16x8*)(la + ra * ROWB + ((pl ^ (ra & 7)) * 16));
-                bh[t] = *(const f16x8*)(lb + rb * ROWB + ((ph ^ (rb & 7)) * 16));
-                bl[t] = *(const f16x8*)(lb + rb * ROWB + ((pl ^ (rb & 7)) * 16));
-            }
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[a], bh[b], acc.w[a][b], 0, 0, 0);
-                    acc.v[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[a], bh[b], acc.v[a][b], 0, 0, 0);
-                    acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[a], bl[b], acc.w[a][b], 0, 0, 0);
-                }
+        for (int i = 0; i < 2 * MT + 4; ++i) {    // a read, and the matrix cores stay busy behind it
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, MT == 4 ? 2 : 1, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070 | NL);  // lgkmcnt(0), vmcnt(NL): f1, and this wave's copies of the next stage
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        read(f0, next, 0);
+        issue(s + 3, buf);
+        multiply(acc, f1);
+#pragma unroll
+        for (int i = 0; i < 2 * MT + 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x010, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        buf = next;
     }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");              // the copies behind the end
     __syncthreads();
 }
 
-// the tile to LDS, times f
-__device__ __forceinline__ void stage_tile(const Acc& acc, float f, float* sm) {
+// f(row, column, value) for the wave's share of a tile
+template <int MT, typename F>
+__device__ __forceinline__ void each(const Acc<MT>& acc, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, q = lane >> 5;
-    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
+    const int wi = (wave >> 1) * 32 * MT, wj = (wave & 1) * 64;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                sm[(wi + 32 * a + 8 * (e >> 2) + 4 * q + (e & 3)) * EP + wj + 32 * b + l31] = (acc.v[a][b][e] + acc.w[a][b][e]) * f;
-    __syncthreads();
+                f(wi + 32 * a + 8 * (e >> 2) + 4 * q + (e & 3), wj + 32 * b + l31, acc.v[a][b][e] + acc.w[a][b][e]);
 }
-// the tile in LDS packed to rows [i0, +128), columns [j0, +128) of `to` (K columns in all)
-__device__ __forceinline__ void put_rows(const float* sm, char* to, int K, int i0, int j0) {
-    for (int u = threadIdx.x; u < 2048; u += 256) {
-        const int i = u >> 4, j = (u & 15) * 8;
-        float v[8];
-        f16x8 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = sm[i * EP + j + e];
-        split8(v, hi, lo);
-        char* d = packed(to, i0 + i, j0 + j, K);
-        *(f16x8*)d = hi;
-        *(f16x8*)(d + 64) = lo;
+
+// The products: what they multiply, and what becomes of `rows` rows of a tile [rows][EP] in LDS that begins at (i0, j0).
+enum Product { XXT, POLY, UPDATE, RESULT };
+
+// tiles of 64 MT x 128 that hold the diagonal of an R x R matrix and what is over it, in blocks of 1024 x 1024 (which share
+// their operands in an XCD's L2): block column after block column
+__device__ __host__ __forceinline__ int tri_count(int cols, int per) {       // tiles of the first `cols` columns of a block on the diagonal
+    int n = 0;
+    for (int j = 0; j < cols; ++j) n += j / per + 1;
+    return n;
+}
+template <int MT>
+__device__ __forceinline__ void tri_tile(int t, int cols, int& ti, int& tj) {
+    constexpr int PER = MT / 2, H = 8 / PER;       // columns of tiles per row of tiles; rows of tiles in a block
+    int J = 0;
+    for (;; ++J) {
+        const int w = cols - 8 * J < 8 ? cols - 8 * J : 8;
+        const int n = J * H * w + tri_count(w, PER);
+        if (t < n) {
+            if (t < J * H * w) {
+                const int blk = t / (H * w), in = t % (H * w);
+                ti = blk * H + in / w;
+                tj = 8 * J + in % w;
+            } else {
+                t -= J * H * w;
+                int j = 0;
+                while (t >= j / PER + 1) t -= j++ / PER + 1;
+                ti = J * H + t;
+                tj = 8 * J + j;
+            }
+            return;
+        }
+        t -= n;
     }
 }
-// its transpose, rows [j0, +128), columns [i0, +128)
-__device__ __forceinline__ void put_cols(const float* sm, char* to, int K, int i0, int j0) {
-    for (int u = threadIdx.x; u < 2048; u += 256) {
-        const int j = u >> 4, i = (u & 15) * 8;
+int tri_tiles(int R, int per) {
+    const int cols = R / TN, h = 8 / per;
+    int n = 0;
+    for (int J = 0; 8 * J < cols; ++J) {
+        const int w = cols - 8 * J < 8 ? cols - 8 * J : 8;
+        n += J * h * w + tri_count(w, per);
+    }
+    return n;
+}
+
+template <int PROD, int MT>
+__device__ __forceinline__ void locate(const Big& p, int tile, int& z, int& i0, int& j0, int tiles) {
+    z = tile / tiles;
+    int t = tile - z * tiles, ti, tj;
+    if constexpr (PROD == XXT || PROD == POLY) {
+        tri_tile<MT>(t, p.R / TN, ti, tj);
+    } else {                                       // eight columns of tiles at a time
+        const int rows = p.L / (64 * MT), cols = p.R / TN, g = t / (8 * rows), w = cols - 8 * g < 8 ? cols - 8 * g : 8, in = t - g * 8 * rows;
+        ti = in / w;
+        tj = 8 * g + in % w;
+    }
+    i0 = ti * 64 * MT;
+    j0 = tj * TN;
+}
+template <int PROD>
+__device__ __forceinline__ float scale_of() {
+    return PROD == XXT ? SA / (SX * SX) : PROD == POLY ? (float)QC * SB / (SA * SA) : PROD == UPDATE ? SX / (SB * SX) : 1.f / (SB * SX);
+}
+
+// columns of ROWS rows in LDS as rows of a packed matrix: four neighbouring threads write 64 bytes of a row, and a wave reads at
+// most two values from a bank
+template <int ROWS, typename F>
+__device__ __forceinline__ void transposed(const float* sm, F to) {
+#pragma unroll 4
+    for (int u = threadIdx.x; u < ROWS * 16; u += 256) {
+        const int j = ROWS == 8 ? u : (u >> 2) & (TN - 1), i = ROWS == 8 ? 0 : ((u >> 9) * 4 + (u & 3)) * 8;
+        char* d = to(i, j);
+        if (!d) continue;
         float v[8];
-        f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sm[(i + e) * EP + j];
-        split8(v, hi, lo);
-        char* d = packed(to, j0 + j, i0 + i, K);
-        *(f16x8*)d = hi;
-        *(f16x8*)(d + 64) = lo;
+        put8(d, v);
     }
 }
 
-// tile t of the upper triangle, counted column by column
-__device__ __forceinline__ void tri(int t, int& i, int& j) {
-    j = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((j + 1) * (j + 2) / 2 <= t) ++j;
-    while (j * (j + 1) / 2 > t) --j;
-    i = t - j * (j + 1) / 2;
-}
-
-__device__ __forceinline__ void gram_end(const Big& p, const Acc& acc, int i0, int j0, int z, float* sm) {
-    char* a = p.a + (size_t)z * p.R * p.R * 4;
-    stage_tile(acc, SA / (SX * SX), sm);
-    put_rows(sm, a, p.R, i0, j0);
-    if (i0 != j0) put_cols(sm, a, p.R, i0, j0);
-}
-
-__device__ __forceinline__ void zero(Acc& acc) {
+template <int PROD, int ROWS, typename T>
+__device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, int j0) {
+    constexpr int N = ROWS == 8 ? 1 : ROWS * 16 / 256, M = N < 8 ? N : 8;     // eight neighbours N times a thread, M of them at a time
+    const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 8;
+    if constexpr (PROD == XXT || PROD == POLY) {
+        char* a = p.a + (size_t)z * p.RA * p.R * 4;
+        char* to = PROD == XXT ? a : p.b + (size_t)z * p.R * p.R * 4;
+        const int cb = j0 / TN;
+        for (int u = 0; u < N; u += M) {
+            f16x8 hi[M], lo[M];
+            if constexpr (PROD == POLY) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+                for (int k = 0; k < M; ++k) {
+                    const int i = row + 16 * (u + k);
+                    if (i >= ROWS || (i0 + i) / TN > cb) continue;
+                    const char* s = packed(a, i0 + i, j0 + col, p.R);
+                    hi[k] = *(const f16x8*)s;
+                    lo[k] = *(const f16x8*)(s + 64);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < M; ++k) {
+                const int i = row + 16 * (u + k);
+                if (i >= ROWS || (i0 + i) / TN > cb) continue;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = sm[i * EP + col + e];
+                    if constexpr (PROD == POLY) {
+                        v[e] += (float)QB * (SB / SA) * ((float)hi[k][e] + (float)lo[k][e]);
+                        if (i0 + i == j0 + col + e) v[e] += (float)QA * SB;
+                        sm[i * EP + col + e] = v[e];
+                    }
+                }
+                put8(packed(to, i0 + i, j0 + col, p.R), v);
+            }
+        }
+        if constexpr (PROD == POLY) __syncthreads();
+        transposed<ROWS>(sm, [&](int i, int j) { return (i0 + i) / TN >= cb ? nullptr : packed(to, j0 + j, i0 + i, p.R); });
+    } else if constexpr (PROD == UPDATE) {                                   // rows: the long side
+        char* xt = p.xt2 + (size_t)z * p.R * p.L * 4;
+        char* x = p.x + (size_t)z * p.RA * p.L * 4;
+#pragma unroll 4
+        for (int i = row; i < ROWS; i += 16) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = sm[i * EP + col + e];
+            put8(packed(xt, i0 + i, j0 + col, p.R), v);
+        }
+        transposed<ROWS>(sm, [&](int i, int j) { return packed(x, j0 + j, i0 + i, p.L); });
+    } else {
+        const Io io = shifted(p.io, (size_t)p.m * p.n * z, sizeof(T));
+        const bool tall = p.m > p.n;
+#pragma unroll 4
+        for (int u = threadIdx.x; u < ROWS * TN; u += 256) {
+            const int i = tall ? u / TN : u % ROWS, j = tall ? u % TN : u / ROWS;
+            if (i0 + i < p.l && j0 + j < p.r)
+                write_o<T>(io, tall ? (size_t)(i0 + i) * p.n + j0 + j : (size_t)(j0 + j) * p.n + i0 + i, sm[i * EP + j]);
+        }
+    }
+}
+
+// Blocks [0, full): a tile each, the card's CUs filled `full / 256` times.  The tiles that are left share the card: `splits`
+// blocks a tile, each with a part of the contraction, whose sums ns_join_kernel adds up.
+template <int PROD, int MT, typename T>
+__global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int tiles, int full, int splits) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int tile = blockIdx.x, split = 0;
+    if (tile < full) tile = (tile & 7) * (full >> 3) + (tile >> 3);          // an XCD's tiles are neighbours
+    else {
+        split = (tile - full) % splits;
+        tile = full + (tile - full) / splits;
+    }
+    const bool whole = (int)blockIdx.x < full || splits == 1;
+    int z, i0, j0;
+    locate<PROD, MT>(p, tile, z, i0, j0, tiles);
+    const char *A, *B;
+    int K;
+    if constexpr (PROD == XXT) {
+        A = B = p.x + (size_t)z * p.RA * p.L * 4;
+        K = p.L;
+    } else if constexpr (PROD == POLY) {
+        A = B = p.a + (size_t)z * p.RA * p.R * 4;
+        K = p.R;
+    } else {
+        A = p.xt + (size_t)z * p.R * p.L * 4;
+        B = p.b + (size_t)z * p.R * p.R * 4;
+        K = p.R;
+    }
+    const int stages = K / KS;
+    const int s0 = whole ? 0 : (int)((long long)stages * split / splits), s1 = whole ? stages : (int)((long long)stages * (split + 1) / splits);
+    Acc<MT> acc;
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[a][b][e] = acc.w[a][b][e] = 0.f;
-}
-
-// A = X X^T; with splits > 1 a share of the contraction, left in the slab
-__global__ __launch_bounds__(256) void ns_xxt_kernel(const Big p) {
-    __shared__ __attribute__((aligned(16))) float sm[TILE * EP];
-    int ti, tj;
-    tri(blockIdx.x, ti, tj);
-    const int z = blockIdx.z, stages = p.L / KS, split = blockIdx.y;
-    const int s0 = (int)((long long)stages * split / p.splits), s1 = (int)((long long)stages * (split + 1) / p.splits);
-    const char* x = p.x + (size_t)z * p.R * p.L * 4;
-    Acc acc;
-    zero(acc);
-    main_loop(acc, x, x, p.L, ti * TILE, tj * TILE, s0, s1, (char*)sm);
-    if (p.splits == 1) {
-        gram_end(p, acc, ti * TILE, tj * TILE, z, sm);
-        return;
+    main_loop(acc, A, B, K, i0, j0, s0, s1, smem);
+    const float f = scale_of<PROD>();
+    if (whole) {
+        float* sm = (float*)smem;
+        each(acc, [&](int i, int j, float v) { sm[i * EP + j] = v * f; });
+        __syncthreads();
+        finish<PROD, 64 * MT, T>(p, sm, z, i0, j0);
+    } else {
+        float* slab = p.slab + ((size_t)(tile - full) * splits + split) * (64 * MT * TN);
+        each(acc, [&](int i, int j, float v) { slab[i * TN + j] = v * f; });
     }
-    float* slab = p.slab + (((size_t)z * gridDim.x + blockIdx.x) * p.splits + split) * (TILE * TILE);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, q = lane >> 5;
-    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                slab[(wi + 32 * a + 8 * (e >> 2) + 4 * q + (e & 3)) * TILE + wj + 32 * b + l31] = acc.v[a][b][e] + acc.w[a][b][e];
 }
-// the shares of 16 rows of a tile, added in order
-__global__ __launch_bounds__(256) void ns_join_kernel(const Big p) {
-    __shared__ float sm[16][EP];
-    int ti, tj;
-    tri(blockIdx.x, ti, tj);
-    const int z = blockIdx.z, row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 8;
-    const int i0 = ti * TILE + blockIdx.y * 16, j0 = tj * TILE;
-    const float* slab = p.slab + ((size_t)z * gridDim.x + blockIdx.x) * p.splits * (TILE * TILE) + (blockIdx.y * 16 + row) * TILE + col;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-        const Pack<float, 4> u = *(const Pack<float, 4>*)(slab + (size_t)s * TILE * TILE);
-        const Pack<float, 4> w = *(const Pack<float, 4>*)(slab + (size_t)s * TILE * TILE + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] += u.v[e];
-            v[4 + e] += w.v[e];
-        }
-    }
-    char* a = p.a + (size_t)z * p.R * p.R * 4;
-    f16x8 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sm[row][col + e] = v[e] *= SA / (SX * SX);
-    split8(v, hi, lo);
-    char* d = packed(a, i0 + row, j0 + col, p.R);
-    *(f16x8*)d = hi;
-    *(f16x8*)(d + 64) = lo;
-    if (ti == tj) return;
+// eight rows of a split tile, its shares added in order
+template <int PROD, int MT, typename T>
+__global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, int full, int splits) {
+    __shared__ __attribute__((aligned(16))) float sm[8 * EP];
+    int z, i0, j0;
+    locate<PROD, MT>(p, full + blockIdx.x, z, i0, j0, tiles);
+    const int i = threadIdx.x >> 5, j = (threadIdx.x & 31) * 4;
+    const float* slab = p.slab + (size_t)blockIdx.x * splits * (64 * MT * TN) + (blockIdx.y * 8 + i) * TN + j;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) v += *(const f32x4*)(slab + (size_t)s * 64 * MT * TN);
+    *(f32x4*)(sm + i * EP + j) = v;
     __syncthreads();
-    const int c = threadIdx.x >> 1, k = (threadIdx.x & 1) * 8;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = sm[k + e][c];
-    split8(v, hi, lo);
-    d = packed(a, j0 + c, i0 + k, p.R);
-    *(f16x8*)d = hi;
-    *(f16x8*)(d + 64) = lo;
-}
-
-// q(A) = a I + b A + c A A
-__global__ __launch_bounds__(256) void ns_poly_kernel(const Big p) {
-    __shared__ __attribute__((aligned(16))) float sm[TILE * EP];
-    int ti, tj;
-    tri(blockIdx.x, ti, tj);
-    const int z = blockIdx.z, i0 = ti * TILE, j0 = tj * TILE;
-    char* a = p.a + (size_t)z * p.R * p.R * 4;
-    char* b = p.b + (size_t)z * p.R * p.R * 4;
-    Acc acc;
-    zero(acc);
-    main_loop(acc, a, a, p.R, i0, j0, 0, p.R / KS, (char*)sm);
-    stage_tile(acc, (float)QC * SB / (SA * SA), sm);
-    for (int u = threadIdx.x; u < 2048; u += 256) {
-        const int i = u >> 4, j = (u & 15) * 8;
-        const char* s = packed(a, i0 + i, j0 + j, p.R);
-        const f16x8 hi = *(const f16x8*)s, lo = *(const f16x8*)(s + 64);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v = sm[i * EP + j + e] + (float)QB * (SB / SA) * ((float)hi[e] + (float)lo[e]);
-            if (i0 + i == j0 + j + e) v += (float)QA * SB;
-            sm[i * EP + j + e] = v;
-        }
-    }
-    __syncthreads();
-    put_rows(sm, b, p.R, i0, j0);
-    if (i0 != j0) put_cols(sm, b, p.R, i0, j0);
-}
-
-// X <- q(A) X: packed both ways, or the result
-template <typename T>
-__global__ __launch_bounds__(256) void ns_update_kernel(const Big p, int last) {
-    __shared__ __attribute__((aligned(16))) float sm[TILE * EP];
-    const int z = blockIdx.z, i0 = blockIdx.x * TILE, j0 = blockIdx.y * TILE;
-    Acc acc;
-    zero(acc);
-    main_loop(acc, p.b + (size_t)z * p.R * p.R * 4, p.xt + (size_t)z * p.R * p.L * 4, p.R, i0, j0, 0, p.R / KS, (char*)sm);
-    if (!last) {
-        stage_tile(acc, SX / (SB * SX), sm);
-        put_rows(sm, p.x + (size_t)z * p.R * p.L * 4, p.L, i0, j0);
-        put_cols(sm, p.xt2 + (size_t)z * p.R * p.L * 4, p.R, i0, j0);
-        return;
-    }
-    stage_tile(acc, 1.f / (SB * SX), sm);
-    const Io io = shifted(p.io, (size_t)p.m * p.n * z, sizeof(T));
-    const bool tall = p.m > p.n;
-    for (int u = threadIdx.x; u < TILE * TILE; u += 256) {
-        const int a = u >> 7, b = u & 127;
-        const int i = tall ? b : a, j = tall ? a : b;
-        if (i0 + i < p.r && j0 + j < p.l)
-            write_o<T>(io, tall ? (size_t)(j0 + j) * p.n + i0 + i : (size_t)(i0 + i) * p.n + j0 + j, sm[i * EP + j]);
-    }
+    finish<PROD, 8, T>(p, sm, z, i0 + blockIdx.y * 8, j0);
 }
 
 // ---------------------------------------------------------------------------------------------- host
+struct Share {
+    int full, rest, splits;
+};
+// `total` tiles of `stages` stages over the CUs: whole rounds, and the rest in parts of 8 stages at least
+Share share(long long total, int stages) {
+    Share s{(int)(total / CUS * CUS), (int)(total % CUS), 1};
+    if (s.rest) {
+        s.splits = CUS / s.rest;
+        if (s.splits > stages / 8) s.splits = stages / 8;
+        if (s.splits > 48) s.splits = 48;
+        if (s.splits < 2) s.splits = 1;
+    }
+    return s;
+}
 struct Layout {
     size_t part, x, xt, xt2, a, b, slab, total;
-    int sub, splits;
+    int sub, mt, R, L, RA, tri, all;
+    Share xxt, poly, update;
 };
-int tiles_of(int R) { return R / TILE * (R / TILE + 1) / 2; }
+Layout layout_of(int nb, int r, int l, int mt) {
+    Layout o{};
+    o.mt = mt;
+    o.R = step::round_up(r, TN);
+    o.L = step::round_up(l, 64 * mt);
+    o.RA = step::round_up(o.R, 64 * mt);
+    o.tri = tri_tiles(o.R, mt / 2);
+    o.all = o.L / (64 * mt) * (o.R / TN);
+    o.xxt = share((long long)o.tri * nb, o.L / KS);
+    o.poly = share((long long)o.tri * nb, o.R / KS);
+    o.update = share((long long)o.all * nb, o.R / KS);
+    return o;
+}
 // workspace of a stack of `batch` matrices with r > 64, `sub` of them at a time
 Layout layout(int batch, int m, int n) {
     const int r = m < n ? m : n, l = m < n ? n : m;
-    const size_t R = step::round_up(r, TILE), L = step::round_up(l, TILE);
-    Layout o;
     const size_t most = (size_t)1 << 28;                           // elements of X at a time
-    const size_t fit = most / (R * L) ? most / (R * L) : 1;
-    o.sub = (int)(fit < (size_t)batch ? fit : (size_t)batch);
-    if (o.sub > 1024) o.sub = 1024;
-    // the contraction of X X^T is split where its tiles do not fill the card twice over, into parts of 8 stages at least
-    const int tiles = tiles_of((int)R) * o.sub, stages = (int)(L / KS);
-    o.splits = 512 / tiles;
-    if (o.splits > stages / 8) o.splits = stages / 8;
-    if (o.splits > 48) o.splits = 48;
-    if (o.splits < 1) o.splits = 1;
+    const size_t fit = most / ((size_t)step::round_up(r, 256) * step::round_up(l, 256));
+    int sub = (int)(fit < (size_t)batch ? fit : (size_t)batch);
+    sub = sub < 1 ? 1 : sub > 1024 ? 1024 : sub;
+    // tiles of 256 rows where they fill the card, of 128 otherwise
+    Layout o = layout_of(sub, r, l, 4);
+    if ((long long)o.all * sub < CUS) o = layout_of(sub, r, l, 2);
+    o.sub = sub;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    o.part = take((size_t)o.sub * NORM_BLOCKS * sizeof(double));
-    o.x = take(o.sub * R * L * 4);
-    o.xt = take(o.sub * R * L * 4);
-    o.xt2 = take(o.sub * R * L * 4);
-    o.a = take(o.sub * R * R * 4);
-    o.b = take(o.sub * R * R * 4);
-    o.slab = take(o.splits > 1 ? (size_t)tiles * o.splits * TILE * TILE * 4 : 0);
+    const size_t R = o.R, L = o.L, RA = o.RA;
+    o.part = take((size_t)sub * NORM_BLOCKS * sizeof(double));
+    o.x = take(sub * RA * L * 4);
+    o.xt = take(sub * R * L * 4);
+    o.xt2 = take(sub * R * L * 4);
+    o.a = take(sub * RA * R * 4);
+    o.b = take(sub * R * R * 4);
+    size_t slab = 0;
+    for (const Share& s : {o.xxt, o.poly, o.update}) {
+        // a smaller last part of the batch is shared out anew: at most 256 parts of tiles either way
+        const size_t parts = s.splits > 1 || sub < batch ? CUS : 0;
+        if (parts > slab) slab = parts;
+    }
+    o.slab = take(slab * 64 * o.mt * TN * 4);
     o.total = at;
     return o;
 }
@@ -687,11 +834,67 @@ int check(const step_ns_item* items, int count) {
     for (int i = 0; i < count; ++i) {
         const step_ns_item& it = items[i];
         STEP_REQUIRE(it.batch >= 1 && it.m >= 1 && it.n >= 1, "step_newton_schulz: item %d: bad shape %d x %d x %d", i, it.batch, it.m, it.n);
-        STEP_REQUIRE(it.m <= (1 << 22) && it.n <= (1 << 22), "step_newton_schulz: item %d: %d x %d is over 2^22 a side", i, it.m, it.n);
+        STEP_REQUIRE(it.m <= (1 << 21) && it.n <= (1 << 21), "step_newton_schulz: item %d: %d x %d is over 2^21 a side", i, it.m, it.n);
         STEP_REQUIRE((it.m < it.n ? it.m : it.n) <= 32768, "step_newton_schulz: item %d: %d x %d is over 32768 on both sides", i, it.m, it.n);
         total += it.batch;
     }
     STEP_REQUIRE(total <= 1 << 24, "step_newton_schulz: %lld matrices", total);
+    return STEP_OK;
+}
+
+template <int PROD, int MT, typename T>
+int product(const Big& p, int tiles, const Share& s, hipStream_t st) {
+    auto kern = ns_product_kernel<PROD, MT, T>;
+    constexpr size_t lds = 3 * (64 * MT + TN) * ROWB;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) {
+        step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
+        return STEP_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL(kern, dim3(s.full + s.rest * s.splits), dim3(256), lds, st, p, tiles, s.full, s.splits);
+    if (s.splits > 1) hipLaunchKernelGGL((ns_join_kernel<PROD, MT, T>), dim3(s.rest, 8 * MT), dim3(256), 0, st, p, tiles, s.full, s.splits);
+    return STEP_OK;
+}
+template <typename T, int MT>
+int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
+    const Layout all = layout(it.batch, it.m, it.n);
+    Big p{};
+    p.m = it.m;
+    p.n = it.n;
+    p.r = it.m < it.n ? it.m : it.n;
+    p.l = it.m < it.n ? it.n : it.m;
+    p.R = all.R;
+    p.L = all.L;
+    p.RA = all.RA;
+    p.eps = eps;
+    p.part = (double*)(base + all.part);
+    p.slab = (float*)(base + all.slab);
+    p.x = base + all.x;
+    p.a = base + all.a;
+    p.b = base + all.b;
+    for (int b0 = 0; b0 < it.batch; b0 += all.sub) {
+        const int nb = it.batch - b0 < all.sub ? it.batch - b0 : all.sub;
+        const Layout o = layout_of(nb, p.r, p.l, MT);
+        const size_t by = (size_t)b0 * it.m * it.n;
+        p.io = io;
+        p.io.g = (const T*)io.g + by;
+        if (io.out) p.io.out = (T*)io.out + by;
+        if (io.momentum) p.io.momentum = io.momentum + by;
+        if (io.param) p.io.param = io.param + by;
+        p.xt = base + all.xt;
+        p.xt2 = base + all.xt2;
+        hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(NORM_BLOCKS, nb), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(ns_pack_kernel<T>, dim3(p.L / 64, p.RA / 64, nb), dim3(256), 0, st, p);
+        for (int s = 0; s < steps; ++s) {
+            int rc = product<XXT, MT, float>(p, o.tri, o.xxt, st);
+            if (rc == STEP_OK) rc = product<POLY, MT, float>(p, o.tri, o.poly, st);
+            if (rc == STEP_OK) rc = s + 1 < steps ? product<UPDATE, MT, float>(p, o.all, o.update, st) : product<RESULT, MT, T>(p, o.all, o.update, st);
+            if (rc != STEP_OK) return rc;
+            char* t = p.xt;
+            p.xt = p.xt2;
+            p.xt2 = t;
+        }
+    }
     return STEP_OK;
 }
 
@@ -731,47 +934,10 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
         }
     }
     for (int i = 0; i < count; ++i) {
-        const step_ns_item& it = items[i];
-        if (small(it.m, it.n)) continue;
-        const Layout o = layout(it.batch, it.m, it.n);
-        Big p{};
-        p.m = it.m;
-        p.n = it.n;
-        p.r = it.m < it.n ? it.m : it.n;
-        p.l = it.m < it.n ? it.n : it.m;
-        p.R = step::round_up(p.r, TILE);
-        p.L = step::round_up(p.l, TILE);
-        p.eps = eps;
-        p.splits = o.splits;
-        char* base = (char*)ws;
-        p.part = (double*)(base + o.part);
-        p.slab = (float*)(base + o.slab);
-        const int tiles = tiles_of(p.R);
-        for (int b0 = 0; b0 < it.batch; b0 += o.sub) {
-            const unsigned nb = (unsigned)(it.batch - b0 < o.sub ? it.batch - b0 : o.sub);
-            const size_t by = (size_t)b0 * it.m * it.n;
-            p.io = io_of(it);
-            p.io.g = (const T*)p.io.g + by;
-            if (p.io.out) p.io.out = (T*)p.io.out + by;
-            if (p.io.momentum) p.io.momentum += by;
-            if (p.io.param) p.io.param += by;
-            p.x = base + o.x;
-            p.xt = base + o.xt;
-            p.xt2 = base + o.xt2;
-            p.a = base + o.a;
-            p.b = base + o.b;
-            hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(NORM_BLOCKS, nb), dim3(256), 0, st, p);
-            hipLaunchKernelGGL(ns_pack_kernel<T>, dim3(p.L / 64, p.R / 64, nb), dim3(256), 0, st, p);
-            for (int s = 0; s < steps; ++s) {
-                hipLaunchKernelGGL(ns_xxt_kernel, dim3(tiles, p.splits, nb), dim3(256), 0, st, p);
-                if (p.splits > 1) hipLaunchKernelGGL(ns_join_kernel, dim3(tiles, TILE / 16, nb), dim3(256), 0, st, p);
-                hipLaunchKernelGGL(ns_poly_kernel, dim3(tiles, 1, nb), dim3(256), 0, st, p);
-                hipLaunchKernelGGL(ns_update_kernel<T>, dim3(p.R / TILE, p.L / TILE, nb), dim3(256), 0, st, p, (int)(s + 1 == steps));
-                char* t = p.xt;
-                p.xt = p.xt2;
-                p.xt2 = t;
-            }
-        }
+        if (small(items[i].m, items[i].n)) continue;
+        const int rc = layout(items[i].batch, items[i].m, items[i].n).mt == 4 ? run_big<T, 4>(items[i], io_of(items[i]), steps, eps, (char*)ws, st)
+                                                                                : run_big<T, 2>(items[i], io_of(items[i]), steps, eps, (char*)ws, st);
+        if (rc != STEP_OK) return rc;
     }
     return step::check_launch("step_newton_schulz");
 }

@@ -347,7 +347,7 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
     double* part = count + 1;
     const Plan pl = plan(classes, dtype, ((uintptr_t)logits & 15) == 0);
     const int blocks = blocks_of(rows, pl);
-    if (mask) hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(1024), 0, st, mask, count, rows);
+    if (mask && !upstream) hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(1024), 0, st, mask, count, rows);
     const Args a{logits, actions, old_logp, advantages, ref_logp, mask, dlogits, logp, mask ? count : nullptr, part,
                  upstream, skip_one, rows, classes, clip_low, clip_high, beta};
     if (dtype == STEP_F32) launch<float>(pl, blocks, a, st);

@@ -84,16 +84,16 @@ class _PolicyLossFn(torch.autograd.Function):
         grad = torch.empty_like(z) if need else None
         ctx.mark_non_differentiable(logp, stats)
         ctx.config = (clip_low, clip_high, beta)
+        nb = _lib.query("step_policy_loss_ws_bytes", rows)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
         if not rows:
             loss.zero_(), stats.zero_()
         else:
-            nb = _lib.query("step_policy_loss_ws_bytes", rows)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
             _lib.call("step_policy_loss", z, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, beta, None, 0,
                       loss, stats, logp, grad, rows, classes, _lib.DTYPES[z.dtype], ws, nb)
         if need:
             ctx.save_for_backward(z, actions, old_logp, advantages, ref_logp, mask)
-            ctx.grad = grad
+            ctx.grad, ctx.ws = grad, ws
         return loss, logp, stats
 
     @staticmethod
@@ -106,10 +106,8 @@ class _PolicyLossFn(torch.autograd.Function):
             grad = torch.empty_like(z)
         rows = z.numel() // z.shape[-1]
         if rows:
-            nb = _lib.query("step_policy_loss_ws_bytes", rows)
-            ws = torch.empty(nb, dtype=torch.uint8, device=z.device)
-            _lib.call("step_policy_loss", z, actions, old_logp, advantages, ref_logp, mask, *ctx.config, g.float().contiguous(),
-                      int(first), None, None, None, grad, rows, z.shape[-1], _lib.DTYPES[z.dtype], ws, nb)
+            _lib.call("step_policy_loss", z, actions, old_logp, advantages, ref_logp, mask, *ctx.config, g.contiguous(),
+                      int(first), None, None, None, grad, rows, z.shape[-1], _lib.DTYPES[z.dtype], ctx.ws, ctx.ws.numel())
         return (grad,) + (None,) * 8
 
 
@@ -143,6 +141,8 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
                 name, " / ".join(str(k)[6:] for k in kinds), getattr(t, "dtype", type(t).__name__)))
         if t.device != logits.device:
             raise _lib.StepHipError("policy_loss: %s is on %s, logits on %s" % (name, t.device, logits.device))
+        if t.dtype is to and t.shape == lead and not t.requires_grad and t.is_contiguous():
+            return t
         try:
             return t.detach().to(to).expand(lead).contiguous()
         except RuntimeError:

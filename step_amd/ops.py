@@ -813,38 +813,43 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         cols = x.shape[-1]
-        xc = x.contiguous()
-        rows = xc.numel() // cols
+        x = x.contiguous()
+        rows = x.numel() // cols
         w = weight.contiguous() if weight is not None else None
         b = bias.contiguous() if bias is not None else None
-        wcode = _lib.DTYPES[w.dtype] if w is not None else _lib.DTYPES[b.dtype] if b is not None else 0
-        y = torch.empty_like(xc)
-        keep = any(ctx.needs_input_grad[:3])
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-        mean, rstd = (stats[0], stats[1]) if keep else (None, None)
+        ctx.wtype = wtype = w.dtype if w is not None else b.dtype if b is not None else torch.float32
+        y = torch.empty_like(x)
+        need = ctx.needs_input_grad
+        mean = rstd = stats = None
+        if need[0] or need[1] or need[2]:
+            stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+            mean = stats.data_ptr()
+            rstd = mean + 4 * rows
+            ctx.save_for_backward(x, w, stats)
         if rows:
-            _lib.call("step_layernorm_fwd", xc, w, b, y, mean, rstd, rows, cols, _lib.DTYPES[x.dtype], wcode, eps)
-        if keep:
-            ctx.save_for_backward(xc, w, stats)
-            ctx.codes = (_lib.DTYPES[x.dtype], wcode)
-            ctx.wtype = w.dtype if w is not None else b.dtype if b is not None else None
+            _lib.call("step_layernorm_fwd", x, w, b, y, mean, rstd, rows, cols, _lib.DTYPES[x.dtype], _lib.DTYPES[wtype], eps)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w, stats = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         cols = x.shape[-1]
         rows = x.numel() // cols
+        dev = x.device
         dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty(cols, dtype=ctx.wtype, device=x.device) if need_w else None
-        db = torch.empty(cols, dtype=ctx.wtype, device=x.device) if need_b else None
+        dw = torch.empty(cols, dtype=ctx.wtype, device=dev) if need_w else None
+        db = torch.empty(cols, dtype=ctx.wtype, device=dev) if need_b else None
         if not rows:
             return dx, dw.zero_() if need_w else None, db.zero_() if need_b else None, None
-        nb = _lib.query("step_layernorm_bwd_ws_bytes", rows, cols) if need_w or need_b else 0
-        ws = _ws(nb, x.device) if nb else None
-        _lib.call("step_layernorm_bwd", dy.contiguous(), x, w, stats[0], stats[1], dx, dw, db, rows, cols, *ctx.codes, ws, nb)
+        nb, ws = 0, None
+        if need_w or need_b:
+            nb = _lib.query("step_layernorm_bwd_ws_bytes", rows, cols)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        mean = stats.data_ptr()
+        _lib.call("step_layernorm_bwd", dy.contiguous(), x, w, mean, mean + 4 * rows, dx, dw, db, rows, cols, _lib.DTYPES[x.dtype],
+                  _lib.DTYPES[ctx.wtype], ws, nb)
         return dx, dw, db, None
 
 

@@ -15,12 +15,11 @@ EPS = 1e-7
 
 def _run(items, dtype, device, steps, eps, momentum=0.0, nesterov=False, lr=0.0, decay=0.0):
     arr = (_lib.NsItem * len(items))(*items)
-    with torch.cuda.device(device):
-        nb = _lib.query("step_newton_schulz_ws_bytes", arr, len(items))
-        if not nb:
-            raise _lib.StepHipError("newton_schulz: %s" % _lib.load().step_last_error().decode())
-        ws = torch.empty(nb, dtype=torch.uint8, device=device)
-        _lib.call("step_newton_schulz", arr, len(items), dtype, steps, eps, momentum, int(nesterov), lr, decay, ws, nb)
+    nb = _lib.query("step_newton_schulz_ws_bytes", arr, len(items))
+    if not nb:
+        raise _lib.StepHipError("newton_schulz: %s" % _lib.load().step_last_error().decode())
+    ws = torch.empty(nb, dtype=torch.uint8, device=device)
+    _lib.call("step_newton_schulz", arr, len(items), dtype, steps, eps, momentum, int(nesterov), lr, decay, ws, nb)
 
 
 def _checked(steps, eps):
@@ -62,7 +61,7 @@ def newton_schulz(g, steps=STEPS, eps=EPS):
             continue
         m, n = c.shape[-2:]
         keep.append(c)
-        items.append(_lib.NsItem(c.data_ptr(), o.data_ptr(), None, None, c.numel() // (m * n), m, n, 1.0))
+        items.append((c.data_ptr(), o.data_ptr(), None, None, c.numel() // (m * n), m, n, 1.0))
     if items:
         _run(items, _lib.DTYPES[gs[0].dtype], gs[0].device, steps, eps)
     return outs if many else outs[0]
@@ -112,31 +111,34 @@ class Muon(torch.optim.Optimizer):
         return loss
 
     def _step_matrices(self, group, mats):
-        items, keep = [], []
+        dev = mats[0].device
         for p in mats:
-            if p.dtype != torch.float32 or p.grad.dtype != torch.float32:
-                raise _lib.StepHipError("Muon keeps fp32 parameters, got %s (gradient %s)" % (p.dtype, p.grad.dtype))
+            g = p.grad
+            if p.dtype is not torch.float32 or g.dtype is not torch.float32:
+                raise _lib.StepHipError("Muon keeps fp32 parameters, got %s (gradient %s)" % (p.dtype, g.dtype))
             if not p.is_cuda:
                 raise _lib.StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % p.device)
-            if p.device != mats[0].device or p.grad.device != p.device:
-                raise _lib.StepHipError("Muon: the parameters of a group lie on %s and %s" % (mats[0].device, p.device))
+            if p.device != dev or g.device != dev:
+                raise _lib.StepHipError("Muon: the parameters of a group lie on %s and %s" % (dev, p.device))
             if not p.is_contiguous():
                 raise _lib.StepHipError("Muon: non-contiguous parameter of shape %s" % (tuple(p.shape),))
+        items, keep, written = [], [], []
         for p in mats:
             state = self.state[p]
-            if "momentum_buffer" not in state:
-                state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-            buf, g = state["momentum_buffer"], p.grad.contiguous()
-            if buf.dtype != torch.float32 or buf.shape != p.shape or buf.device != p.device or not buf.is_contiguous():
+            buf = state.get("momentum_buffer")
+            if buf is None:
+                buf = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            elif buf.dtype is not torch.float32 or buf.shape != p.shape or buf.device != dev or not buf.is_contiguous():
                 raise _lib.StepHipError("Muon: momentum buffer %s %s does not fit its parameter" % (buf.dtype, tuple(buf.shape)))
+            g = p.grad.contiguous()
             m = p.shape[0]
             n = p.numel() // m
             keep.append(g)
-            items.append(_lib.NsItem(g.data_ptr(), None, buf.data_ptr(), p.data_ptr(), 1, m, n, math.sqrt(max(1.0, m / n))))
-        _run(items, 0, mats[0].device, group["steps"], group["eps"], group["momentum"], group["nesterov"], group["lr"], group["weight_decay"])
-        for p in mats:                            # written behind torch's back: caches and saved tensors go by the version
-            torch.autograd.graph.increment_version(p)
-            torch.autograd.graph.increment_version(self.state[p]["momentum_buffer"])
+            written += (p, buf)
+            items.append((g.data_ptr(), None, buf.data_ptr(), p.data_ptr(), 1, m, n, math.sqrt(m / n) if m > n else 1.0))
+        _run(items, 0, dev, group["steps"], group["eps"], group["momentum"], group["nesterov"], group["lr"], group["weight_decay"])
+        # written behind torch's back: caches and saved tensors go by the version
+        torch.autograd.graph.increment_version(written)
 
     def _step_rest(self, group, rest):
         lr = group["lr"] if group["adam_lr"] is None else group["adam_lr"]
