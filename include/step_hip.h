@@ -531,8 +531,7 @@ int step_layernorm_bwd(const void* dy, const void* x, const void* w, const float
  *          / max(#live, 1)
  * logits (rows, classes) contiguous of type `dtype`; actions int64, old_logp / advantages / ref_logp (nullable: no KL term)
  * fp32, mask bytes (nullable: every row is live), one per row.  loss[1], stats[3] = {policy part, KL, share of clipped rows},
- * logp[rows] (0 in masked rows) fp32; dlogits (nullable) like logits and at the same place within 16 bytes.  A masked row is
- * not read.  An action outside [0, classes) of a live row makes the loss and the row's gradient NaN; nothing is read there.
+ * logp[rows] (0 in masked rows) fp32; dlogits (nullable) like logits.  A masked row is not read.  An action outside [0, classes) of a live row makes the loss and the row's gradient NaN; nothing is read there.
  * With `upstream` (a device scalar) only dlogits is written, times *upstream; skip_one: nothing is done where *upstream is
  * exactly 1 (the caller's dlogits already holds that gradient), and ws is the one that the call without `upstream` left (it
  * holds the number of live rows).  ws: step_policy_loss_ws_bytes(rows).                                       */

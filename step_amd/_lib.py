@@ -142,17 +142,6 @@ def load():
     return _lib
 
 
-def _ptr(t):
-    if t is None:
-        return None
-    if not t.is_cuda:
-        raise StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no "
-                           "CPU path" % t.device)
-    if not t.is_contiguous():
-        raise StepHipError("non-contiguous tensor passed to the C ABI")
-    return t.data_ptr()
-
-
 def stream(device=None):
     index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)     # (no Stream object: 0.3 us a launch instead of 2 to 9)
@@ -162,26 +151,30 @@ def call(name, *args):
     """Call an int-returning entry point on torch's current stream OF THE TENSORS' DEVICE; raise on error.
     Every tensor argument must live on one GPU; the launch (and any per-device kernel attribute the library
     sets) happens with that GPU current, whatever torch's current device is."""
-    lib = load()
-    dev = None
+    lib = _lib or load()
+    index = -1
     conv = []
     for a in args:
-        if a is None or isinstance(a, torch.Tensor):
-            conv.append(_ptr(a))
-            if a is not None:
-                if dev is None:
-                    dev = a.device
-                elif a.device != dev:
-                    raise StepHipError("%s: tensor arguments on different devices (%s and %s)"
-                                       % (name, dev, a.device))
+        if isinstance(a, torch.Tensor):
+            i = a.get_device()
+            if i != index or i < 0:
+                if i < 0:
+                    raise StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % a.device)
+                if index >= 0:
+                    raise StepHipError("%s: tensor arguments on different devices (cuda:%d and %s)" % (name, index, a.device))
+                index = i
+            if not a.is_contiguous():
+                raise StepHipError("non-contiguous tensor passed to the C ABI")
+            conv.append(a.data_ptr())
         else:
             conv.append(a)
     fn = getattr(lib, name)
-    if dev is None or dev.index == torch.cuda.current_device():
-        rc = fn(*conv, stream(dev))
+    current = torch.cuda.current_device()
+    if index < 0 or index == current:
+        rc = fn(*conv, torch._C._cuda_getCurrentRawStream(current))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*conv, stream(dev))
+        with torch.cuda.device(index):
+            rc = fn(*conv, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         raise StepHipError("%s failed (%d): %s" % (name, rc, lib.step_last_error().decode()))
 

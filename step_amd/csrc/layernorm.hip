@@ -4,62 +4,44 @@
 //   t = dy w:  dx = r (t - mean t - xhat mean(t xhat)),  dw = SUM_rows dy xhat,  db = SUM_rows dy
 //
 // Memory-bound both ways: forward 2 and backward 3 elements moved per element.  A row stays in the registers of the G
-// threads that share it between the statistics and the result, so each tensor is moved once.  G is the smallest of
-// 8 / 64 / 256 / 1024 whose threads hold the row in at most two 16-byte packs each (plan() below): short rows share a
-// wave, long ones have a block.  The statistics are combined pairwise from (count, mean, sum of squared deviations),
-// which loses nothing to a mean far from zero and takes one reduction instead of two.
-// dw and db: a block keeps its columns' sums in fp32 registers over all its rows, writes one line of partial sums, and a
-// second launch adds the lines in a fixed order - the same bits every time, no atomics.
+// threads that share it between the statistics and the result, so each tensor is moved once.  G is 8, 64, 256 or 1024, the
+// smallest whose threads hold the row (plan() below): up to 4096 16-bit columns a wave has a row to itself and needs no
+// barrier; sums over a wave are data-parallel-primitive adds (no LDS).  Two sums in the forward, the mean's
+// and that of the squared deviations from it, the second with the rest of the mean: nothing is lost to a mean far from zero.
+// dw and db: a thread keeps its columns' sums in fp32 registers over all its rows; a block adds its waves' in order and
+// writes one line of partial sums, and a second launch adds the lines in a fixed order - the same bits every time, no
+// atomics.
 #include "rows.h"
 
 namespace {
 using namespace step;
 
-struct Stat {
-    float n, mean, m2;
-};
-// pairwise combination of two sets of values; the same result whichever half a thread is in is not needed: the first
-// thread's value is broadcast
-__device__ __forceinline__ Stat combine(const Stat a, const Stat b) {
-    const float n = a.n + b.n;
-    const float f = n > 0.f ? b.n / n : 0.f;
-    const float d = b.mean - a.mean;
-    return Stat{n, a.mean + d * f, a.m2 + b.m2 + d * d * (a.n * f)};
-}
-
+// sums of a and b over the 8 or 64 threads that share a row, the same bits in all of them
 template <int G>
-__device__ __forceinline__ Stat group_stat(Stat s, Stat* sm) {
-#pragma unroll
-    for (int o = 1; o < (G < 64 ? G : 64); o <<= 1) {
-        const Stat t{__shfl_xor(s.n, o, 64), __shfl_xor(s.mean, o, 64), __shfl_xor(s.m2, o, 64)};
-        s = combine(s, t);
-    }
-    if constexpr (G <= 64) {
-        const int src = (threadIdx.x & 63) & ~(G - 1);
-        return Stat{s.n, __shfl(s.mean, src, 64), __shfl(s.m2, src, 64)};
-    } else {
-        __syncthreads();                       // the last row's readers are done with sm
-        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = s;
-        __syncthreads();
-        Stat r = sm[0];
-#pragma unroll
-        for (int i = 1; i < G / 64; ++i) r = combine(r, sm[i]);
-        return r;
+__device__ __forceinline__ void wave_sum2(float& a, float& b) {
+    a += dpp<0xb1>(a);             // quad_perm 1 0 3 2
+    b += dpp<0xb1>(b);
+    a += dpp<0x4e>(a);             // quad_perm 2 3 0 1
+    b += dpp<0x4e>(b);
+    a += dpp<0x141>(a);            // row_half_mirror
+    b += dpp<0x141>(b);
+    if constexpr (G >= 64) {
+        a += dpp<0x140>(a);        // row_mirror: sums of 16
+        b += dpp<0x140>(b);
+        a = rows16(a, [](float x, float y) { return x + y; });
+        b = rows16(b, [](float x, float y) { return x + y; });
     }
 }
-
+// the same over G threads that may be several waves (then the whole block comes here): `sm` the group's 2 G / 64 floats, which the
+// next call does not use
 template <int G>
 __device__ __forceinline__ void group_sum2(float& a, float& b, float* sm) {
-#pragma unroll
-    for (int o = 1; o < (G < 64 ? G : 64); o <<= 1) {
-        a += __shfl_xor(a, o, 64);
-        b += __shfl_xor(b, o, 64);
-    }
+    wave_sum2<G>(a, b);
     if constexpr (G > 64) {
-        __syncthreads();
+        const int wave = (threadIdx.x % G) >> 6;
         if ((threadIdx.x & 63) == 0) {
-            sm[2 * (threadIdx.x >> 6)] = a;
-            sm[2 * (threadIdx.x >> 6) + 1] = b;
+            sm[2 * wave] = a;
+            sm[2 * wave + 1] = b;
         }
         __syncthreads();
         a = sm[0];
@@ -72,139 +54,130 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float* sm) {
     }
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* p, float* v) {
-    const Pack<T, VEC> q = *(const Pack<T, VEC>*)p;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = (float)q.v[e];
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, const float* v) {
-    Pack<T, VEC> q;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) q.v[e] = (T)v[e];          // the result's only rounding
-    *(Pack<T, VEC>*)p = q;
-}
-
-template <typename T, int VEC, int NV, int G>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void ln_fwd_kernel(const T* __restrict__ x, const void* __restrict__ w,
-                                                                   const void* __restrict__ b, T* __restrict__ y,
+// a block: 256 threads, or one row's 1024
+template <typename T, typename W, int VEC, int NV, int G>
+__global__ __launch_bounds__(G > 256 ? G : 256) void ln_fwd_kernel(const T* __restrict__ x, const W* __restrict__ w,
+                                                                   const W* __restrict__ b, T* __restrict__ y,
                                                                    float* __restrict__ mean, float* __restrict__ rstd,
-                                                                   long long rows, int cols, int wdtype, float eps) {
-    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
-    __shared__ Stat sm[G > 64 ? G / 64 : 1];
+                                                                   long long rows, int cols, float eps) {
+    constexpr int BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
+    constexpr int SUMS = G > 64 ? 2 * BLOCK / 64 : 1;
+    __shared__ float sm[2 * SUMS];
+    float* const mine = sm + (G > 64 ? threadIdx.x / G * (2 * G / 64) : 0);
     const int lane = threadIdx.x % G;
-    float wv[NV][VEC], bv[NV][VEC];
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int c = (i * G + lane) * VEC + e;
-            wv[i][e] = w && c < cols ? load_as(w, c, wdtype) : 1.f;
-            bv[i][e] = b && c < cols ? load_as(b, c, wdtype) : 0.f;
-        }
+    const float inv_c = 1.f / (float)cols;
+    Pack<W, VEC> wv[NV], bv[NV];
+    const Columns<VEC, NV, G> own{cols, lane};
+    if (w) own.load(wv, w);
+    if (b) own.load(bv, b);
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
         const long long row = r0 + threadIdx.x / G;
         const bool live = row < rows;
-        const T* xr = x + (size_t)row * cols;
-        float v[NV][VEC];
-        float s = 0.f;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * VEC;
-            if (live && c < cols) {
-                load_vec<T, VEC>(xr + c, v[i]);
-                n += VEC;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) s += v[i][e];
-            }
-        }
-        Stat st{(float)n, n ? s / (float)n : 0.f, 0.f};
+        Pack<T, VEC> v[NV];
+        own.load(v, x + (size_t)(live ? row : rows - 1) * cols);
+        own.fill(v, (T)0.f);
+        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live && (i * G + lane) * VEC < cols)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float d = v[i][e] - st.mean;
-                    st.m2 += d * d;
-                }
-        st = group_stat<G>(st, sm);
-        const float inv = 1.f / sqrtf(st.m2 / (float)cols + eps);
+            for (int e = 0; e < VEC; e += 2) {               // two chains
+                s1 += (float)v[i].v[e];
+                if (e + 1 < VEC) s2 += (float)v[i].v[e + 1];
+            }
+        s1 += s2;
+        s2 = 0.f;
+        group_sum2<G>(s1, s2, mine);
+        float mu = s1 * inv_c;
+        s1 = s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = own.mine(i, e) ? (float)v[i].v[e] - mu : 0.f;
+                s1 += d;
+                s2 += d * d;
+            }
+        group_sum2<G>(s1, s2, mine + SUMS);
+        s1 *= inv_c;                                         // the rest of the mean
+        const float inv = 1.f / sqrtf(fmaxf(s2 * inv_c - s1 * s1, 0.f) + eps);
+        mu += s1;
         if (!live) continue;
         if (lane == 0 && mean) {
-            mean[row] = st.mean;
+            mean[row] = mu;
             rstd[row] = inv;
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * VEC;
-            if (c < cols) {
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[i][e] = (v[i][e] - st.mean) * inv * wv[i][e] + bv[i][e];
-                store_vec<T, VEC>(y + (size_t)row * cols + c, v[i]);
+            for (int e = 0; e < VEC; ++e) {
+                float o = ((float)v[i].v[e] - mu) * inv;
+                if (w) o *= (float)wv[i].v[e];
+                if (b) o += (float)bv[i].v[e];
+                v[i].v[e] = (T)o;                            // the result's only rounding
             }
-        }
+        own.store(y + (size_t)row * cols, v);
     }
 }
 
-template <typename T, int VEC, int NV, int G>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
-                                                                   const void* __restrict__ w,
-                                                                   const float* __restrict__ mean,
+// a block: 512 threads, or one row's 1024
+template <typename T, typename W, int VEC, int NV, int G>
+__global__ __launch_bounds__(G > 512 ? G : 512) void ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+                                                                   const W* __restrict__ w, const float* __restrict__ mean,
                                                                    const float* __restrict__ rstd, T* __restrict__ dx,
-                                                                   float* __restrict__ part, long long rows, int cols,
-                                                                   int wdtype) {
-    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
-    __shared__ float sm[G > 64 ? 2 * G / 64 : 1];
-    __shared__ float acc[RPB > 1 ? BLOCK * NV * VEC : 1];
+                                                                   float* __restrict__ part, long long rows, int cols) {
+    constexpr int BLOCK = G > 512 ? G : 512, RPB = BLOCK / G, SUMS = G > 64 ? 2 * BLOCK / 64 : 1;
+    __shared__ float sm[2 * SUMS];
+    __shared__ float acc[RPB > 1 ? G * NV * VEC : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
-    float wv[NV][VEC], dw[NV][VEC], db[NV][VEC];
+    Pack<W, VEC> wv[NV];
+    const Columns<VEC, NV, G> own{cols, lane};
+    if (w) own.load(wv, w);
+    float dw[NV][VEC], db[NV][VEC];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int c = (i * G + lane) * VEC + e;
-            wv[i][e] = w && c < cols ? load_as(w, c, wdtype) : 1.f;
-            dw[i][e] = db[i][e] = 0.f;
-        }
+        for (int e = 0; e < VEC; ++e) dw[i][e] = db[i][e] = 0.f;
     const float inv_c = 1.f / (float)cols;
+    int turn = 0;
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
         const long long row = r0 + group;
         const bool live = row < rows;
-        const size_t at = (size_t)row * cols;
-        const float mu = live ? mean[row] : 0.f, inv = live ? rstd[row] : 0.f;
-        float g[NV][VEC], xh[NV][VEC];
+        const size_t at = (size_t)(live ? row : rows - 1) * cols;
+        const float mu = mean[live ? row : rows - 1], inv = rstd[live ? row : rows - 1];
+        Pack<T, VEC> g[NV], v[NV];
+        own.load(g, dy + at);
+        own.load(v, x + at);
+        own.fill(g, (T)0.f);
+        if (!live)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) g[i].v[e] = (T)0.f;
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * G + lane) * VEC;
-            if (live && c < cols) {
-                load_vec<T, VEC>(dy + at + c, g[i]);
-                load_vec<T, VEC>(x + at + c, xh[i]);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    xh[i][e] = (xh[i][e] - mu) * inv;
-                    dw[i][e] += g[i][e] * xh[i][e];
-                    db[i][e] += g[i][e];
-                    g[i][e] *= wv[i][e];
-                    s1 += g[i][e];
-                    s2 += g[i][e] * xh[i][e];
-                }
+            for (int e = 0; e < VEC; ++e) {                  // (dy is 0 where the column is not its own)
+                const float d = (float)g[i].v[e], xh = ((float)v[i].v[e] - mu) * inv, t = w ? d * (float)wv[i].v[e] : d;
+                dw[i][e] += d * xh;
+                db[i][e] += d;
+                s1 += t;
+                s2 += t * xh;
             }
-        }
         if (dx) {
-            group_sum2<G>(s1, s2, sm);
+            group_sum2<G>(s1, s2, sm + (G > 64 ? turn * SUMS + group * (2 * G / 64) : 0));
+            turn ^= 1;
             s1 *= inv_c;
             s2 *= inv_c;
+            if (live) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * G + lane) * VEC;
-                if (live && c < cols) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) g[i][e] = inv * (g[i][e] - s1 - xh[i][e] * s2);
-                    store_vec<T, VEC>(dx + at + c, g[i]);
-                }
+                for (int i = 0; i < NV; ++i)
+        #pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const float d = (float)g[i].v[e], xh = ((float)v[i].v[e] - mu) * inv, t = w ? d * (float)wv[i].v[e] : d;
+                        g[i].v[e] = (T)(inv * (t - s1 - xh * s2));
+                    }
+                own.store(dx + at, g);
             }
         }
     }
@@ -213,26 +186,38 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void ln_bwd_kernel(const T* __re
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         if constexpr (RPB > 1) {
-            __syncthreads();
+            if constexpr (G < 64)                            // a wave's rows first
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+                for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    acc[group * G * NV * VEC + (i * G + lane) * VEC + e] = which ? db[i][e] : dw[i][e];
-            __syncthreads();
-            for (int c = threadIdx.x; c < cols; c += BLOCK) {
-                float s = 0.f;
-                for (int r = 0; r < RPB; ++r) s += acc[r * G * NV * VEC + c];
-                line[which * cols + c] = s;
+                    for (int e = 0; e < VEC; ++e)
+#pragma unroll
+                        for (int o = G; o < 64; o <<= 1) {
+                            if (which) db[i][e] += __shfl_xor(db[i][e], o, 64);
+                            else dw[i][e] += __shfl_xor(dw[i][e], o, 64);
+                        }
+            constexpr int GROUP = G < 64 ? 64 : G;
+            for (int k = 0; k < BLOCK / GROUP; ++k) {        // then the block's, in order
+                if ((int)threadIdx.x / GROUP == k && threadIdx.x % GROUP < G)
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (own.mine(i, e)) {
+                                const int c = own.at(i) + e;
+                                const float t = which ? db[i][e] : dw[i][e];
+                                acc[c] = k ? acc[c] + t : t;
+                            }
+                __syncthreads();
             }
+            for (int c = threadIdx.x; c < cols; c += BLOCK) line[which * cols + c] = acc[c];
+            __syncthreads();
         } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int c = (i * G + lane) * VEC + e;
-                    if (c < cols) line[which * cols + c] = which ? db[i][e] : dw[i][e];
-                }
+                for (int e = 0; e < VEC; ++e)
+                    if (own.mine(i, e)) line[which * cols + own.at(i) + e] = which ? db[i][e] : dw[i][e];
         }
     }
 }
@@ -258,43 +243,38 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
     }
 }
 
-// Rows longer than 1024 threads hold: the row is read again for the result, the columns' sums are a pass of their own.
+// Rows longer than 1024 threads hold: the row is read again for each sum and the result, the columns' sums are a pass of their
+// own.
 template <typename T>
 __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, const void* __restrict__ w,
                                                            const void* __restrict__ b, T* __restrict__ y,
                                                            float* __restrict__ mean, float* __restrict__ rstd,
                                                            long long rows, int cols, int wdtype, float eps) {
-    __shared__ Stat sm[16];
+    __shared__ float sm[64];
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + (size_t)row * cols;
-        Stat st{0.f, 0.f, 0.f};
-        for (int c0 = 0; c0 < cols; c0 += 8192) {                // eight values a thread, then one combination
-            float v[8];
-            float s = 0.f, n = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = c0 + e * 1024 + threadIdx.x;
-                if (c < cols) {
-                    v[e] = (float)xr[c];
-                    s += v[e];
-                    n += 1.f;
-                }
-            }
-            Stat t{n, n > 0.f ? s / n : 0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c0 + e * 1024 + (int)threadIdx.x < cols) t.m2 += (v[e] - t.mean) * (v[e] - t.mean);
-            st = combine(st, t);
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x; c < cols; c += 1024) s1 += (float)xr[c];
+        group_sum2<1024>(s1, s2, sm);
+        float mu = s1 / (float)cols;
+        s1 = s2 = 0.f;
+        for (int c = threadIdx.x; c < cols; c += 1024) {
+            const float d = (float)xr[c] - mu;
+            s1 += d;
+            s2 += d * d;
         }
-        st = group_stat<1024>(st, sm);
-        const float inv = 1.f / sqrtf(st.m2 / (float)cols + eps);
+        group_sum2<1024>(s1, s2, sm + 32);
+        s1 /= (float)cols;
+        const float inv = 1.f / sqrtf(fmaxf(s2 / (float)cols - s1 * s1, 0.f) + eps);
+        mu += s1;
         if (threadIdx.x == 0 && mean) {
-            mean[row] = st.mean;
+            mean[row] = mu;
             rstd[row] = inv;
         }
         for (int c = threadIdx.x; c < cols; c += 1024)
-            y[(size_t)row * cols + c] = (T)(((float)xr[c] - st.mean) * inv * (w ? load_as(w, c, wdtype) : 1.f) +
+            y[(size_t)row * cols + c] = (T)(((float)xr[c] - mu) * inv * (w ? load_as(w, c, wdtype) : 1.f) +
                                             (b ? load_as(b, c, wdtype) : 0.f));
+        __syncthreads();
     }
 }
 
@@ -303,7 +283,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* __restrict__
                                                            const void* __restrict__ w, const float* __restrict__ mean,
                                                            const float* __restrict__ rstd, T* __restrict__ dx,
                                                            long long rows, int cols, int wdtype) {
-    __shared__ float sm[32];
+    __shared__ float sm[64];
+    int turn = 0;
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const size_t at = (size_t)row * cols;
         const float mu = mean[row], inv = rstd[row];
@@ -313,7 +294,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_kernel(const T* __restrict__
             s1 += t;
             s2 += t * (((float)x[at + c] - mu) * inv);
         }
-        group_sum2<1024>(s1, s2, sm);
+        group_sum2<1024>(s1, s2, sm + 32 * turn);
+        turn ^= 1;
         s1 /= (float)cols;
         s2 /= (float)cols;
         for (int c = threadIdx.x; c < cols; c += 1024) {
@@ -348,69 +330,69 @@ __global__ __launch_bounds__(1024) void ln_cols_long_kernel(const T* __restrict_
     }
 }
 
+constexpr int MAX_LINES = 512;
+
 struct Plan {
-    int g, nv, vec;                 // g 0: a row is too long for the registers of 1024 threads
+    int g, nv, vec;                 // threads per row, packs per thread, elements of a pack; g 0: too long for the registers of 1024 threads
 };
-// Threads per row and packs per thread.  16-byte packs where every row starts at a multiple of 16 bytes; single elements
-// otherwise (their columns must be the same for all rows: a thread keeps its columns' gradient sums).
-Plan plan(int cols, int dtype, bool aligned) {
+// The fewest threads whose registers hold the row.  The forward keeps a row's elements as they are, and the weights: 8 packs a
+// thread (16384 x 4096 bf16 on a wave a row: 47 us, 5.7 TB/s; on a block of 256 threads 48).  The backward also keeps two sums
+// per column, 32 elements a thread are the most without spills (8192 x 8192 bf16: 84 us at 256 threads x 32, 100 at 1024 x 8).
+// Rows shorter than a pack are read by elements.
+constexpr int NV_FWD = 8, NV_1024 = 4;              // (1024 threads have half the registers)
+constexpr int nv_bwd(int vec) { return 32 / vec; }
+Plan plan(int cols, int dtype, bool fwd) {
     const int vec = 16 / elem_bytes(dtype);
-    if (aligned && cols % vec == 0) {
-        for (int g : {8, 64, 256, 1024})
-            for (int nv : {1, 2})
-                if (cols <= g * nv * vec) return Plan{g, nv, vec};
-    } else {
-        for (int g : {8, 64, 256, 1024})
-            for (int nv : {2, 8})
-                if (cols <= g * nv) return Plan{g, nv, 1};
-        if (cols <= 16384) return Plan{1024, 16, 1};
-    }
+    if (cols < vec) return Plan{8, 1, 1};
+    if (cols <= 8 * vec) return Plan{8, 1, vec};
+    const int most = fwd ? NV_FWD : nv_bwd(vec);
+    for (int g : {64, 256})
+        if (cols <= (long long)g * most * vec) return Plan{g, step::ceil_div(cols, g * vec), vec};
+    if (fwd && cols <= 1024 * NV_1024 * vec) return Plan{1024, step::ceil_div(cols, 1024 * vec), vec};
+    if (!fwd && cols <= 512 * most * vec) return Plan{512, step::ceil_div(cols, 512 * vec), vec};
     return Plan{0, 0, 0};
 }
 int lines_of(long long rows, const Plan& p) {
     if (!p.g) return (int)(rows < 16 * 64 ? (rows + 15) / 16 : 64);
-    const int rpb = p.g < 256 ? 256 / p.g : 1, cap = p.g == 1024 ? 256 : 512;
-    const long long blocks = (rows + rpb - 1) / rpb;
+    // a block a CU where a thread has many elements (the rows in flight are enough and the lines of sums are fewer), two
+    // otherwise; as many rows a group as leave 128 blocks, up to four, or adding the lines takes longer than the rows
+    const int rpb = p.g < 512 ? 512 / p.g : 1, cap = p.nv * p.vec > 16 ? MAX_LINES / 2 : MAX_LINES;
+    const long long one = (rows + rpb - 1) / rpb, blocks = one / 4 > 128 ? one / 4 : one < 128 ? one : 128;
     return (int)(blocks < cap ? blocks : cap);
 }
 
-bool aligned16(const void* a, const void* b, const void* c) {
-    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
-}
-
-template <typename F>
-int with_type(int dtype, F f) {
-    if (dtype == STEP_F32) return f(float());
-    if (dtype == STEP_BF16) return f(bf16());
-    return f(f16());
-}
-
-// calls f(integral constants VEC, NV, G) for a plan of element type T
+// calls f(integral constants VEC, NV, G) for a plan
 template <int V>
 using Int = std::integral_constant<int, V>;
-template <typename T, typename F>
+template <int VEC, int G, int FROM, int MOST, typename F>
+void with_nv(int nv, F f) {
+    if (nv == FROM) f(Int<VEC>(), Int<FROM>(), Int<G>());
+    else if constexpr (FROM < MOST) with_nv<VEC, G, FROM + 1, MOST>(nv, f);
+}
+template <typename T, bool FWD, typename F>
 void with_plan(const Plan& p, F f) {
-    constexpr int VEC = 16 / (int)sizeof(T);
-    auto groups = [&](auto vec, auto nv) {
-        if (p.g == 8) f(vec, nv, Int<8>());
-        else if (p.g == 64) f(vec, nv, Int<64>());
-        else if (p.g == 256) f(vec, nv, Int<256>());
-        else f(vec, nv, Int<1024>());
-    };
-    if (p.vec > 1) {
-        if (p.nv == 1) groups(Int<VEC>(), Int<1>());
-        else groups(Int<VEC>(), Int<2>());
-    } else if (p.nv == 2) groups(Int<1>(), Int<2>());
-    else if (p.nv == 8) groups(Int<1>(), Int<8>());
-    else f(Int<1>(), Int<16>(), Int<1024>());
+    constexpr int VEC = 16 / (int)sizeof(T), MOST = FWD ? NV_FWD : nv_bwd(VEC);
+    if (p.vec == 1) with_nv<1, 8, 1, 1>(p.nv, f);
+    else if (p.g == 8) with_nv<VEC, 8, 1, 1>(p.nv, f);
+    else if (p.g == 64) with_nv<VEC, 64, 1, MOST>(p.nv, f);
+    else if (p.g == 256) with_nv<VEC, 256, MOST / 4 + 1, MOST>(p.nv, f);      // fewer fit in 64 threads
+    else if constexpr (FWD) with_nv<VEC, 1024, MOST / 4 + 1, NV_1024>(p.nv, f);
+    else with_nv<VEC, 512, MOST / 2 + 1, MOST>(p.nv, f);
+}
+// calls f(T(), W()) for the rows' and the weights' types: the same, or fp32 weights
+template <typename F>
+int with_types(int dtype, int wdtype, F f) {
+    if (dtype == STEP_F32) return f(float(), float());
+    if (dtype == STEP_BF16) return wdtype == STEP_F32 ? f(bf16(), float()) : f(bf16(), bf16());
+    return wdtype == STEP_F32 ? f(f16(), float()) : f(f16(), f16());
 }
 
 }  // namespace
 
 extern "C" size_t step_layernorm_bwd_ws_bytes(long long rows, int cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    // the same for every type and alignment: 512 lines at most
-    const long long lines = rows < 512 ? rows : 512;
+    // the same for every type and alignment
+    const long long lines = rows < MAX_LINES ? rows : MAX_LINES;
     return (size_t)lines * 2 * cols * sizeof(float);
 }
 
@@ -419,24 +401,28 @@ extern "C" int step_layernorm_fwd(const void* x, const void* w, const void* b, v
     STEP_REQUIRE(x && y, "step_layernorm_fwd: null pointer");
     STEP_REQUIRE(rows >= 1 && cols >= 1, "step_layernorm_fwd: bad shape rows=%lld cols=%d", rows, cols);
     STEP_REQUIRE(elem_bytes(dtype) && elem_bytes(wdtype), "step_layernorm_fwd: unknown type %d / %d", dtype, wdtype);
+    STEP_REQUIRE(wdtype == STEP_F32 || wdtype == dtype, "step_layernorm_fwd: weights of type %d beside rows of type %d", wdtype, dtype);
     STEP_REQUIRE((mean == nullptr) == (rstd == nullptr), "step_layernorm_fwd: mean and rstd come together");
     hipStream_t st = (hipStream_t)stream;
-    const Plan p = plan(cols, dtype, aligned16(x, y, nullptr));
-    with_type(dtype, [&](auto t) {
+    const Plan p = plan(cols, dtype, true);
+    with_types(dtype, wdtype, [&](auto t, auto u) {
         using T = decltype(t);
+        using W = decltype(u);
         if (!p.g) {
             const long long blocks = rows < 1024 ? rows : 1024;
             hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)blocks), dim3(1024), 0, st, (const T*)x, w, b, (T*)y, mean,
                                rstd, rows, cols, wdtype, eps);
             return 0;
         }
-        with_plan<T>(p, [&](auto vec, auto nv, auto g) {
-            constexpr int G = decltype(g)::value, BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
-            const long long need = (rows + RPB - 1) / RPB, cap = 4096;
-            hipLaunchKernelGGL((ln_fwd_kernel<T, decltype(vec)::value, decltype(nv)::value, G>),
-                               dim3((unsigned)(need < cap ? need : cap)), dim3(BLOCK), 0, st, (const T*)x, w, b, (T*)y, mean,
-                               rstd, rows, cols, wdtype, eps);
-        });
+        auto go = [&](auto vec, auto nv, auto g) {
+            constexpr int G = decltype(g)::value, BLOCK = G > 256 ? G : 256, RPB = BLOCK / G;
+            // four rows a thread group or more, once every CU has two blocks: the weights are read once for them
+            const long long need = (rows + RPB - 1) / RPB, cap = need / 4 < 512 ? 512 : need / 4 < 2048 ? need / 4 : 2048;
+            hipLaunchKernelGGL((ln_fwd_kernel<T, W, decltype(vec)::value, decltype(nv)::value, G>),
+                               dim3((unsigned)(need < cap ? need : cap)), dim3(BLOCK), 0, st, (const T*)x, (const W*)w,
+                               (const W*)b, (T*)y, mean, rstd, rows, cols, eps);
+        };
+        with_plan<T, true>(p, go);
         return 0;
     });
     return step::check_launch("step_layernorm_fwd");
@@ -448,6 +434,7 @@ extern "C" int step_layernorm_bwd(const void* dy, const void* x, const void* w, 
     STEP_REQUIRE(dy && x && mean && rstd, "step_layernorm_bwd: null pointer");
     STEP_REQUIRE(rows >= 1 && cols >= 1, "step_layernorm_bwd: bad shape rows=%lld cols=%d", rows, cols);
     STEP_REQUIRE(elem_bytes(dtype) && elem_bytes(wdtype), "step_layernorm_bwd: unknown type %d / %d", dtype, wdtype);
+    STEP_REQUIRE(wdtype == STEP_F32 || wdtype == dtype, "step_layernorm_bwd: weights of type %d beside rows of type %d", wdtype, dtype);
     const bool sums = dw || db;
     STEP_REQUIRE(!sums || ws, "step_layernorm_bwd: null workspace");
     if (sums && ws_bytes < step_layernorm_bwd_ws_bytes(rows, cols)) {
@@ -456,11 +443,12 @@ extern "C" int step_layernorm_bwd(const void* dy, const void* x, const void* w, 
     }
     if (!dx && !sums) return STEP_OK;
     hipStream_t st = (hipStream_t)stream;
-    const Plan p = plan(cols, dtype, aligned16(dy, x, dx));
+    const Plan p = plan(cols, dtype, false);
     const int lines = lines_of(rows, p);
     float* part = sums ? (float*)ws : nullptr;
-    with_type(dtype, [&](auto t) {
+    with_types(dtype, wdtype, [&](auto t, auto u) {
         using T = decltype(t);
+        using W = decltype(u);
         if (!p.g) {
             const long long blocks = rows < 1024 ? rows : 1024;
             if (dx)
@@ -471,11 +459,12 @@ extern "C" int step_layernorm_bwd(const void* dy, const void* x, const void* w, 
                                    (const T*)dy, (const T*)x, mean, rstd, part, rows, cols);
             return 0;
         }
-        with_plan<T>(p, [&](auto vec, auto nv, auto g) {
-            constexpr int G = decltype(g)::value, BLOCK = G < 256 ? 256 : G;
-            hipLaunchKernelGGL((ln_bwd_kernel<T, decltype(vec)::value, decltype(nv)::value, G>), dim3(lines), dim3(BLOCK), 0,
-                               st, (const T*)dy, (const T*)x, w, mean, rstd, (T*)dx, part, rows, cols, wdtype);
-        });
+        auto go = [&](auto vec, auto nv, auto g) {
+            constexpr int G = decltype(g)::value, BLOCK = G > 512 ? G : 512;
+            hipLaunchKernelGGL((ln_bwd_kernel<T, W, decltype(vec)::value, decltype(nv)::value, G>), dim3(lines), dim3(BLOCK), 0,
+                               st, (const T*)dy, (const T*)x, (const W*)w, mean, rstd, (T*)dx, part, rows, cols);
+        };
+        with_plan<T, false>(p, go);
         return 0;
     });
     if (sums)

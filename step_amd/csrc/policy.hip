@@ -18,7 +18,10 @@ using namespace step;
 
 constexpr float L2E = 1.4426950408889634f, L2E_REST = 1.92596299e-8f;
 constexpr double LN2 = 0.69314718055994530942;
+constexpr float LN2_HI = 0.6931471824645996f;            // ln 2 in fp32, and what is left
+constexpr double LN2_LO = -1.904654299957768e-09;
 constexpr int MAX_BLOCKS = 2048;
+
 
 struct Args {
     const void* logits;
@@ -35,27 +38,6 @@ struct Args {
     int classes;
     double clip_low, clip_high, beta;   // a clipped ratio's 1.2 in fp32 is off by 4e-8, the same way in every row
 };
-
-// 16 bytes of a row, -inf outside it; a pack that the row fills only in part is read by elements, so nothing outside the
-// row is touched
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_pack(const T* row, int e0, int classes) {
-    if (e0 >= 0 && e0 + N <= classes) return *(const Pack<T, N>*)(row + e0);
-    Pack<T, N> q;
-#pragma unroll
-    for (int e = 0; e < N; ++e) q.v[e] = e0 + e >= 0 && e0 + e < classes ? row[e0 + e] : (T)(-__builtin_inff());
-    return q;
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_pack(T* row, int e0, int classes, const Pack<T, N> q) {
-    if (e0 >= 0 && e0 + N <= classes) {
-        *(Pack<T, N>*)(row + e0) = q;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (e0 + e >= 0 && e0 + e < classes) row[e0 + e] = q.v[e];
-}
 
 // maximum and sum of exponentials about it, joined over the G threads of a row, in base 2: m is the row's largest logit
 // times log2 e, rounded once and from there on exact, an element's exponent x log2 e - m is one fused operation
@@ -76,7 +58,6 @@ __device__ __forceinline__ Soft join(const Soft w, Soft* sm) {
     if constexpr (G <= 64) {
         return w;
     } else {
-        __syncthreads();
         if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = w;
         __syncthreads();
         Soft r = sm[0];
@@ -90,17 +71,56 @@ __device__ __forceinline__ Soft join(const Soft w, Soft* sm) {
     }
 }
 
+// exp and log2 in fp64 for a row's scalars, from their series: a third of the registers and of the time that the general
+// functions take, which one thread of a block spends while the others wait.
+// log2 s = e + log2 m, s = m 2^e with m in [sqrt 1/2, sqrt 2): log m = 2 atanh t, t = (m - 1) / (m + 1), |t| <= 0.172, to t^13:
+// the rest is under 2 t^15 / 15 = 5e-13.  (s is 1 or more, or NaN, or comes from a row that allows nothing, where m is -inf.)
+__device__ __forceinline__ double log2_of(float s) {
+    int e = __builtin_amdgcn_frexp_expf(s);
+    float m = __builtin_amdgcn_frexp_mantf(s);
+    if (m < 0.70710678f) {
+        m *= 2.f;
+        --e;
+    }
+    const double d = (double)m + 1.0;
+    double r = __builtin_amdgcn_rcp(d);
+    r = r * (2.0 - d * r);
+    r = r * (2.0 - d * r);
+    const double t = ((double)m - 1.0) * r, u = t * t;
+    const double a = 1.0 + u * (1.0 / 3 + u * (1.0 / 5 + u * (1.0 / 7 + u * (1.0 / 9 + u * (1.0 / 11 + u * (1.0 / 13))))));
+    return (double)e + (2.0 / LN2) * (t * a);
+}
+// e^x = 2^n e^r, |r| <= ln 2 / 2, to r^10: the rest is under 0.347^11 / 11! = 3e-13; beyond e^+-700 infinity and 0, NaN stays
+__device__ __forceinline__ double exp_of64(double x) {
+    if (!(x < 700.0)) return x == x ? (double)__builtin_inff() : x;
+    if (x < -700.0) return 0.0;
+    const double n = __builtin_rint(x * (1.0 / LN2));
+    const double r = __builtin_fma(n, -(LN2_LO), __builtin_fma(n, -(double)LN2_HI, x));   // n LN2_HI is exact
+    double p = 1.0 / 3628800;
+    p = p * r + 1.0 / 362880;
+    p = p * r + 1.0 / 40320;
+    p = p * r + 1.0 / 5040;
+    p = p * r + 1.0 / 720;
+    p = p * r + 1.0 / 120;
+    p = p * r + 1.0 / 24;
+    p = p * r + 1.0 / 6;
+    p = p * r + 0.5;
+    p = p * r + 1.0;
+    p = p * r + 1.0;
+    return __builtin_ldexp(p, (int)n);
+}
+
 // the row's scalars: returns dL/dlp / count (times the upstream gradient), adds the row to the block's sums
 __device__ __forceinline__ float row_scalars(const Args& p, long long row, Soft f, float za, bool valid, double count,
                                              double* sums) {
-    const double lp = valid ? (double)za - ((double)f.m + log2((double)f.s)) * LN2 : (double)__builtin_nanf("");
-    const double a = p.adv[row], ratio = exp(lp - (double)p.old_logp[row]);
+    const double lp = valid ? (double)za - ((double)f.m + log2_of(f.s)) * LN2 : (double)__builtin_nanf("");
+    const double a = p.adv[row], ratio = exp_of64(lp - (double)p.old_logp[row]);
     const double lo = 1.0 - p.clip_low, hi = 1.0 + p.clip_high;
     const double o1 = ratio * a, o2 = (ratio > hi ? hi : ratio < lo ? lo : ratio) * a;   // a NaN stays one
     const bool clipped = o1 > o2;
     double slope = clipped ? 0.0 : -o1, kl = 0.0;
     if (p.ref) {
-        const double d = (double)p.ref[row] - lp, e = exp(d);
+        const double d = (double)p.ref[row] - lp, e = exp_of64(d);
         kl = e - d - 1.0;
         slope += p.beta * (1.0 - e);
     }
@@ -112,17 +132,34 @@ __device__ __forceinline__ float row_scalars(const Args& p, long long row, Soft 
     return (float)(slope / count);
 }
 
+// -coef softmax(z) for the elements of a pack; the drawn action's + coef comes afterwards
 template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> gradient_of(const Pack<T, N> z, int e0, long long action, float m, float inv_s,
-                                                  float coef) {
+__device__ __forceinline__ Pack<T, N> gradient_of(const Pack<T, N>& z, float m, float scale) {
     Pack<T, N> g;
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        float v = -coef * (exp_of((float)z.v[e], m) * inv_s);
-        if (e0 + e == action) v += coef;
-        g.v[e] = (T)v;                                       // the gradient's only rounding
-    }
+    for (int e = 0; e < N; ++e) g.v[e] = (T)(exp_of((float)z.v[e], m) * scale);       // the gradient's only rounding
     return g;
+}
+// adds N elements to a thread's maximum and sum: their largest first, so that nothing overflows
+template <typename T, int N>
+__device__ __forceinline__ void add_to(Soft& f, const Pack<T, N>* q, int packs) {
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < packs; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, (float)q[k].v[e]);
+    m = fmaxf(f.m, m * L2E);
+    const float m0 = finite_or_0(m);
+    float s0 = f.s * exp_of(f.m - m0), s1 = 0.f;             // two chains
+#pragma unroll
+    for (int k = 0; k < packs; ++k)
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            s0 += exp_for_sum((float)q[k].v[e], m0);
+            if (e + 1 < N) s1 += exp_for_sum((float)q[k].v[e + 1], m0);
+        }
+    f.s = s0 + s1;
+    f.m = m;
 }
 
 // sums of one block -> part[block]; the threads that hold none pass zeros
@@ -143,70 +180,87 @@ __device__ __forceinline__ void block_sums(double* part, double* sums) {
     }
 }
 
-// NV packs of 16 bytes a thread; NV = 0: the row is read twice
-template <typename T, int G, int NV>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void policy_kernel(const Args p) {
-    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G, N = 16 / (int)sizeof(T), KEEP = NV ? NV : 1;
-    __shared__ Soft sm[G > 64 ? G / 64 : 1];
+// what was computed from a pack is computed again behind this: a row's elements stay in registers as they are, and not as
+// floats beside
+template <typename T, int N>
+__device__ __forceinline__ void forget(Pack<T, N>& v) {
+    if constexpr (sizeof(T) < 4 && sizeof(v) == 16) {
+        u32x4 q = __builtin_bit_cast(u32x4, v);
+        asm volatile("" : "+v"(q));
+        v = __builtin_bit_cast(Pack<T, N>, q);
+    }
+}
+
+// G threads a row, NV packs of N elements a thread (the last LAST of them may not fit); NV = 0: the row is read twice
+template <typename T, int N, int NV, int LAST, int G>
+__global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_kernel(const Args p) {
+    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G, KEEP = NV ? NV : 1;
+    __shared__ Soft sm[2][G > 64 ? G / 64 : 1];
     __shared__ float coef_s;
     if (p.upstream && p.skip_one && *p.upstream == 1.f) return;
     const int lane = threadIdx.x % G;
+    const Columns<N, KEEP, G, LAST> own{p.classes, lane};
     const double live_rows = p.count ? *p.count : (double)p.rows, count = live_rows > 1.0 ? live_rows : 1.0;
     double sums[3] = {0.0, 0.0, 0.0};
+    int turn = 0;
     for (long long r0 = (long long)blockIdx.x * RPB; r0 < p.rows; r0 += (long long)gridDim.x * RPB) {
         const long long row = r0 + threadIdx.x / G;
         if (G <= 64 && row >= p.rows) continue;              // (whole blocks share a row otherwise)
         const T* z = (const T*)p.logits + (size_t)row * p.classes;
         T* g = p.dlogits ? (T*)p.dlogits + (size_t)row * p.classes : nullptr;
-        const int shift = (int)(((uintptr_t)z & 15) / sizeof(T));
-        const int packs = (shift + p.classes + N - 1) / N;
         if (p.mask && !p.mask[row]) {
             if (lane == 0 && !p.upstream) p.logp[row] = 0.f;
             if (g) {
                 Pack<T, N> zero;
 #pragma unroll
                 for (int e = 0; e < N; ++e) zero.v[e] = (T)0.f;
-                for (int i = lane; i < packs; i += G) store_pack<T, N>(g, i * N - shift, p.classes, zero);
+                for (int c = lane * N; c < p.classes; c += G * N) store_pack<T, N>(g + (c < p.classes - N ? c : p.classes - N), zero);
             }
             continue;
         }
-        const long long action = p.actions[row];
-        const bool valid = action >= 0 && action < p.classes;
-        const float za = lane == 0 && valid ? (float)z[action] : 0.f;
+        const long long a64 = p.actions[row];
+        const bool valid = a64 >= 0 && a64 < p.classes;
+        const int action = valid ? (int)a64 : -1;
         Pack<T, N> v[KEEP];
         Soft f{-__builtin_inff(), 0.f};
+        if constexpr (NV > 0) own.load(v, z);
+        const float za = lane == 0 && valid ? (float)z[action] : 0.f;
+        auto larger = [](float a, float b) { return fmaxf(a, b); };
+        auto sum = [](float a, float b) { return a + b; };
         if constexpr (NV > 0) {
+            own.fill(v, (T)-__builtin_inff());
+            constexpr int U = N == 4 && NV % 2 == 0 ? 2 : 1; // eight elements at a time
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = load_pack<T, N>(z, (i * G + lane) * N - shift, p.classes);
+            for (int i = 0; i < NV; i += U) {
+                add_to<T, N>(f, v + i, U);
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < N; ++e) f.m = fmaxf(f.m, (float)v[i].v[e]);
-            f.m = group_wave_reduce<G>(f.m, [](float a, float b) { return fmaxf(a, b); }) * L2E;
-            const float m0 = finite_or_0(f.m);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < N; ++e) f.s += exp_for_sum((float)v[i].v[e], m0);
-        } else {
-            for (int i = lane; i < packs; i += G) {
-                const Pack<T, N> q = load_pack<T, N>(z, i * N - shift, p.classes);
-                float m = -__builtin_inff();
-#pragma unroll
-                for (int e = 0; e < N; ++e) m = fmaxf(m, (float)q.v[e]);
-                m = fmaxf(f.m, m * L2E);
-                const float m0 = finite_or_0(m);
-                f.s *= exp_of(f.m - m0);
-#pragma unroll
-                for (int e = 0; e < N; ++e) f.s += exp_for_sum((float)q.v[e], m0);
-                f.m = m;
+                for (int k = 0; k < U; ++k) forget(v[i + k]);
             }
-            const float m = group_wave_reduce<G>(f.m, [](float a, float b) { return fmaxf(a, b); });
-            f.s *= exp_of(f.m - finite_or_0(m));
-            f.m = m;
+        } else {
+            constexpr int U = 8;                             // packs in flight
+            for (int c0 = 0; c0 < p.classes; c0 += U * G * N) {
+                Pack<T, N> q[U];
+                int at[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const int c = c0 + (k * G + lane) * N;
+                    at[k] = c < p.classes - N ? c : p.classes - N;
+                    q[k] = load_pack<T, N>(z + at[k]);
+                }
+                if (c0 + U * G * N > p.classes)
+#pragma unroll
+                    for (int k = 0; k < U; ++k)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) q[k].v[e] = at[k] + e >= c0 + (k * G + lane) * N ? q[k].v[e] : (T)-__builtin_inff();
+#pragma unroll
+                for (int k = 0; k < U; ++k) add_to<T, N>(f, q + k, 1);
+            }
         }
-        f.s = group_wave_reduce<G>(f.s, [](float a, float b) { return a + b; });
-        f = join<G>(f, sm);
+        const float m = wave_reduce<G>(f.m, larger);
+        f.s = wave_reduce<G>(f.s * exp_of(f.m - finite_or_0(m)), sum);
+        f.m = m;
+        f = join<G>(f, sm[turn]);
+        turn ^= 1;
         float coef;
         if constexpr (G <= 64) {
             double add[3] = {0.0, 0.0, 0.0};
@@ -219,20 +273,29 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void policy_kernel(const Args p)
             coef = coef_s;
         }
         if (!g) continue;
-        const float inv_s = 1.f / f.s;
+        const float scale = -coef / f.s;
         if constexpr (NV > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e0 = (i * G + lane) * N - shift;
-                if (e0 < p.classes) store_pack<T, N>(g, e0, p.classes, gradient_of<T, N>(v[i], e0, action, f.m, inv_s, coef));
-            }
+            for (int i = 0; i < NV; ++i) own.store(g, i, gradient_of<T, N>(v[i], f.m, scale));
         } else {
-            for (int i = lane; i < packs; i += G) {
-                const int e0 = i * N - shift;
-                const Pack<T, N> q = load_pack<T, N>(z, e0, p.classes);
-                store_pack<T, N>(g, e0, p.classes, gradient_of<T, N>(q, e0, action, f.m, inv_s, coef));
+            constexpr int U = 8;
+            for (int c0 = 0; c0 < p.classes; c0 += U * G * N) {
+                Pack<T, N> q[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const int c = c0 + (k * G + lane) * N;
+                    q[k] = load_pack<T, N>(z + (c < p.classes - N ? c : p.classes - N));
+                }
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const int c = c0 + (k * G + lane) * N;
+                    if (c < p.classes) store_pack<T, N>(g + (c < p.classes - N ? c : p.classes - N), gradient_of<T, N>(q[k], f.m, scale));
+                }
             }
+            __syncthreads();                                 // (packs overlap at the row's end)
         }
+        // the thread that wrote the action's element writes it once more
+        if (valid && lane == action / N % G) g[action] = (T)(exp_of((float)z[action], f.m) * scale + coef);
     }
     if (!p.upstream) block_sums<BLOCK>(p.part, sums);
 }
@@ -284,40 +347,44 @@ __global__ __launch_bounds__(256) void policy_finish_kernel(const double* __rest
 }
 
 struct Plan {
-    int g, nv;
+    int g, nv, vec;                                          // nv 0: too long for the registers of 1024 threads
 };
-Plan plan(int classes, int dtype, bool aligned) {
+// The fewest threads whose registers hold the row: few waves wait for each other, more rows are in a CU at a time, and the rows
+// of a wave share the time of their scalars (65536 x 1000 bf16: 71 us with a wave a row).  Rows shorter than a pack are read by
+// elements.
+Plan plan(int classes, int dtype) {
     const int n = 16 / elem_bytes(dtype);
-    // packs that the row touches at most, whatever 16-byte boundary it starts behind
-    const long long packs = aligned && classes % n == 0 ? classes / n : ((long long)classes + 2 * n - 2) / n;
-    const Plan all[] = {{8, 1}, {64, 1}, {64, 4}, {256, 4}, {1024, 2}, {1024, 4}, {1024, 8}, {1024, 16}};
-    for (const Plan& p : all)
-        if (packs <= (long long)p.g * p.nv) return p;
-    return Plan{1024, 0};
+    if (classes < n) return Plan{8, 1, 1};
+    const int packs = (classes - 1) / n + 1;
+    for (int g : {8, 16, 64, 256, 512, 1024})
+        if (packs <= (g < 64 ? 8 : 16) * g) {
+            const int nv = (packs + g - 1) / g;
+            return Plan{g, nv <= 4 ? nv : (nv + 1) / 2 * 2, n};
+        }
+    return Plan{1024, 0, n};
 }
 int blocks_of(long long rows, const Plan& p) {
-    const int rpb = p.g < 256 ? 256 / p.g : 1, cap = p.g == 1024 ? 512 : MAX_BLOCKS;
+    const int rpb = p.g < 256 ? 256 / p.g : 1, cap = p.g == 1024 ? 512 : p.g == 512 ? 1024 : MAX_BLOCKS;
     const long long need = (rows + rpb - 1) / rpb;
     return (int)(need < cap ? need : cap);
 }
 
+template <typename T, int N, int G, int NV, int MOST>
+void launch_nv(int nv, int blocks, const Args& a, hipStream_t st) {
+    if (nv == NV) hipLaunchKernelGGL((policy_kernel<T, N, NV, NV <= 4 ? 1 : 2, G>), dim3(blocks), dim3(G < 256 ? 256 : G), 0, st, a);
+    else if constexpr (NV < MOST) launch_nv<T, N, G, NV < 4 ? NV + 1 : NV + 2, MOST>(nv, blocks, a, st);
+}
 template <typename T>
 void launch(const Plan& pl, int blocks, const Args& a, hipStream_t st) {
-#define STEP_POLICY(G, NV)                                                                                     \
-    if (pl.g == G && pl.nv == NV) {                                                                            \
-        hipLaunchKernelGGL((policy_kernel<T, G, NV>), dim3(blocks), dim3(G < 256 ? 256 : G), 0, st, a);        \
-        return;                                                                                                \
-    }
-    STEP_POLICY(8, 1)
-    STEP_POLICY(64, 1)
-    STEP_POLICY(64, 4)
-    STEP_POLICY(256, 4)
-    STEP_POLICY(1024, 2)
-    STEP_POLICY(1024, 4)
-    STEP_POLICY(1024, 8)
-    STEP_POLICY(1024, 16)
-    STEP_POLICY(1024, 0)
-#undef STEP_POLICY
+    constexpr int N = 16 / (int)sizeof(T);
+    if (pl.vec == 1) launch_nv<T, 1, 8, 1, 1>(1, blocks, a, st);
+    else if (pl.g == 8) launch_nv<T, N, 8, 1, 8>(pl.nv, blocks, a, st);
+    else if (pl.g == 16) launch_nv<T, N, 16, 6, 8>(pl.nv, blocks, a, st);      // fewer fit in 8 threads, and so on
+    else if (pl.g == 64) launch_nv<T, N, 64, 3, 16>(pl.nv, blocks, a, st);
+    else if (pl.g == 256) launch_nv<T, N, 256, 6, 16>(pl.nv, blocks, a, st);
+    else if (pl.g == 512) launch_nv<T, N, 512, 10, 16>(pl.nv, blocks, a, st);
+    else if (pl.nv) launch_nv<T, N, 1024, 10, 16>(pl.nv, blocks, a, st);
+    else hipLaunchKernelGGL((policy_kernel<T, N, 0, 1, 1024>), dim3(blocks), dim3(1024), 0, st, a);
 }
 
 }  // namespace
@@ -335,9 +402,7 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
     STEP_REQUIRE(rows >= 1 && classes >= 1 && classes <= 0x7fffff00, "step_policy_loss: bad shape rows=%lld classes=%d", rows, classes);
     STEP_REQUIRE(elem_bytes(dtype), "step_policy_loss: unknown type %d", dtype);
     STEP_REQUIRE(upstream ? dlogits != nullptr : loss && stats && logp, "step_policy_loss: null output");
-    STEP_REQUIRE(!dlogits || (((uintptr_t)logits ^ (uintptr_t)dlogits) & 15) == 0,
-                 "step_policy_loss: logits and dlogits lie differently to 16 bytes");
-    STEP_REQUIRE(((uintptr_t)logits & (elem_bytes(dtype) - 1)) == 0, "step_policy_loss: logits lie across elements");
+    STEP_REQUIRE((((uintptr_t)logits | (uintptr_t)dlogits) & (elem_bytes(dtype) - 1)) == 0, "step_policy_loss: logits or dlogits lie across elements");
     if (ws_bytes < step_policy_loss_ws_bytes(rows)) {
         step::set_error("step_policy_loss: workspace %zu < %zu bytes", ws_bytes, step_policy_loss_ws_bytes(rows));
         return STEP_ERR_WORKSPACE;
@@ -345,7 +410,7 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
     hipStream_t st = (hipStream_t)stream;
     double* count = (double*)ws;
     double* part = count + 1;
-    const Plan pl = plan(classes, dtype, ((uintptr_t)logits & 15) == 0);
+    const Plan pl = plan(classes, dtype);
     const int blocks = blocks_of(rows, pl);
     if (mask && !upstream) hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(1024), 0, st, mask, count, rows);
     const Args a{logits, actions, old_logp, advantages, ref_logp, mask, dlogits, logp, mask ? count : nullptr, part,

@@ -74,8 +74,6 @@ class _PolicyLossFn(torch.autograd.Function):
         classes = logits.shape[-1]
         rows = logits.numel() // classes
         z = logits.contiguous()
-        if z.data_ptr() % 16:                     # the gradient, which starts at 16 bytes, is written in the same packs
-            z = z.clone()
         dev = z.device
         loss = torch.empty((), dtype=torch.float32, device=dev)
         stats = torch.empty(3, dtype=torch.float32, device=dev)
