@@ -55,24 +55,30 @@ __device__ __forceinline__ void write_o(const Io& io, size_t at, float o) {
 
 // ---------------------------------------------------------------------------------------------- r <= 64
 constexpr int S_ITEMS = 24;                       // matrices' descriptions that fit a launch's arguments
-constexpr int S_P = 68;                           // row pitch of a 64 x 64 fp64 matrix in LDS: 8 rows in different banks
+constexpr int S_P = 66;                           // row pitch of a 64 x 64 fp64 matrix in LDS: 16 rows begin 4 banks apart
 
 struct SmallItem {
     Io io;
-    int m, n, first, chunks, width;               // first matrix of the item; chunks of `width` columns of the long side
+    int m, n, chunks, width;                      // chunks of `width` columns of the long side
     size_t slab, p;                               // offsets in the workspace, in doubles
 };
 struct SmallArgs {
+    int first[S_ITEMS];                           // first matrix of each item; behind the items more than all
     SmallItem item[S_ITEMS];
-    int items, total, steps, max_chunks;
+    int items, total, steps, max_chunks, max_parts;   // (parts: 64 columns each, of ns_apply_kernel)
     float eps;
     double* ws;
 };
 // item and element offset of matrix z
 __device__ __forceinline__ const SmallItem& find(const SmallArgs& p, int z, int& local) {
-    int i = 0;
-    while (i + 1 < p.items && p.item[i + 1].first <= z) ++i;
-    local = z - p.item[i].first;
+    int i = 0, first = 0;
+#pragma unroll
+    for (int k = 1; k < S_ITEMS; ++k)             // (all read at once, and not one after the other)
+        if (p.first[k] <= z) {
+            i = k;
+            first = p.first[k];
+        }
+    local = z - first;
     return p.item[i];
 }
 __device__ __forceinline__ Io shifted(Io io, size_t by, int bytes) {
@@ -83,34 +89,55 @@ __device__ __forceinline__ Io shifted(Io io, size_t by, int bytes) {
     return io;
 }
 
-// one chunk of columns: its part of G G^T, upper 16 x 16 tiles, [10][256] doubles
+constexpr int GRAM_WAVES = 12;
+// sixteen columns c0 .. c0 + 15 of the short side's rows 16 t + i16: element (t, s) is column c0 + 4 q + s
+template <typename T, bool UPDATE>
+__device__ __forceinline__ void read_columns(float (&u)[4][4], const Io& io, int m, int n, int r, int c0, int c1, int i16, int q) {
+    const bool tall = m > n;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int row = 16 * t + i16, col = c0 + 4 * q;
+        if (!tall && row < r && col + 4 <= c1) {             // four neighbours
+            const size_t at = (size_t)row * n + col;
+            const Pack<T, 4> g = load_pack<T, 4>((const T*)io.g + at);
+            Pack<float, 4> v{{(float)g.v[0], (float)g.v[1], (float)g.v[2], (float)g.v[3]}};
+            if (io.momentum) {
+                Pack<float, 4> w = load_pack<float, 4>(io.momentum + at);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    if (UPDATE) w.v[s] = io.mu * w.v[s] + v.v[s];
+                    v.v[s] = io.nesterov ? v.v[s] + io.mu * w.v[s] : w.v[s];
+                }
+                if (UPDATE) store_pack<float, 4>(io.momentum + at, w);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) u[t][s] = v.v[s];
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                u[t][s] = row < r && col + s < c1 ? read_u<T>(io, tall ? (size_t)(col + s) * n + row : (size_t)row * n + col + s, UPDATE) : 0.f;
+        }
+    }
+}
+
+// one chunk of columns: its part of G G^T, upper 16 x 16 tiles, [10][256] doubles; 16 columns a wave at a time
 template <typename T>
-__global__ __launch_bounds__(256) void ns_gram_kernel(const SmallArgs p) {
-    __shared__ double sm[10 * 256];
+__global__ __launch_bounds__(64 * GRAM_WAVES) void ns_gram_kernel(const SmallArgs p) {
+    __shared__ double sm[4][2560];
     const int z = blockIdx.x / p.max_chunks, chunk = blockIdx.x % p.max_chunks;
     int local;
     const SmallItem& it = find(p, z, local);
     if (chunk >= it.chunks) return;
-    const bool tall = it.m > it.n;
-    const int r = tall ? it.n : it.m, l = tall ? it.m : it.n;
+    const int r = min(it.m, it.n), l = max(it.m, it.n);
     const Io io = shifted(it.io, (size_t)local * it.m * it.n, sizeof(T));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
     f64x4 acc[10];
 #pragma unroll
     for (int t = 0; t < 10; ++t) acc[t] = f64x4{0, 0, 0, 0};
     const int c1 = min(l, (chunk + 1) * it.width);
-    for (int c0 = chunk * it.width + 16 * wave; c0 < c1; c0 += 64) {
-        // 16 columns; step s takes the columns 4 q + s (the order of a contraction is free)
-        float u[4][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int row = 16 * t + i16, col = c0 + 4 * q + s;
-                u[t][s] = row < r && col < c1
-                              ? read_u<T>(io, tall ? (size_t)col * it.n + row : (size_t)row * it.n + col, true)
-                              : 0.f;
-            }
+    for (int c0 = chunk * it.width + 16 * wave; c0 < c1; c0 += 16 * GRAM_WAVES) {
+        float u[4][4];                                       // step s takes the columns 4 q + s: the order of a contraction is free
+        read_columns<T, true>(u, io, it.m, it.n, r, c0, c1, i16, q);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             int k = 0;
@@ -122,48 +149,76 @@ __global__ __launch_bounds__(256) void ns_gram_kernel(const SmallArgs p) {
                         acc[k] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[a][s], (double)u[b][s], acc[k], 0, 0, 0);
         }
     }
-    // the four waves' sums, in order
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w)
+    // the waves' sums in four columns of three, in order
+    for (int w = 0; w < GRAM_WAVES / 4; ++w) {
+        if (wave / 4 == w)
 #pragma unroll
             for (int t = 0; t < 10; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int at = t * 256 + i * 64 + lane;
-                    sm[at] = w ? sm[at] + acc[t][i] : acc[t][i];
+                    double& d = sm[wave & 3][t * 256 + i * 64 + lane];
+                    d = w ? d + acc[t][i] : acc[t][i];
                 }
         __syncthreads();
     }
     double* slab = p.ws + it.slab + ((size_t)local * it.chunks + chunk) * 2560;
-    for (int e = threadIdx.x; e < 2560; e += 256) slab[e] = sm[e];
+    for (int e = threadIdx.x; e < 2560; e += 64 * GRAM_WAVES) slab[e] = (sm[0][e] + sm[1][e]) + (sm[2][e] + sm[3][e]);
 }
 
-// C = X Y for commuting symmetric X, Y in LDS: tiles on and over the diagonal, mirrored; f(i, j, value) stores
-template <typename F>
-__device__ __forceinline__ void sym_product(const double* X, const double* Y, int nt, F f) {
+// C = X Y for commuting symmetric X, Y of 16 NT rows in LDS: one tile on or over the diagonal a wave, mirrored; f(i, j, value) stores
+template <int NT, typename F>
+__device__ __forceinline__ void sym_product(const double* X, const double* Y, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
-    int k = 0;
-    for (int a = 0; a < nt; ++a)
-        for (int b = a; b < nt; ++b, ++k) {
-            if (k % 8 != wave) continue;
-            f64x4 c{0, 0, 0, 0}, d{0, 0, 0, 0};
-            for (int s = 0; s < 4 * nt; s += 2) {
-                c = __builtin_amdgcn_mfma_f64_16x16x4f64(X[(16 * a + i16) * S_P + 4 * s + q], Y[(16 * b + i16) * S_P + 4 * s + q], c, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f64_16x16x4f64(X[(16 * a + i16) * S_P + 4 * s + 4 + q], Y[(16 * b + i16) * S_P + 4 * s + 4 + q], d, 0, 0, 0);
-            }
+    if (wave >= NT * (NT + 1) / 2) return;
+    int a = 0, b = wave;
+    while (b >= NT) b -= NT - ++a;                           // row a of the triangle has NT - a tiles
+    const double* x = X + (16 * a + i16) * S_P + q;
+    const double* y = Y + (16 * b + i16) * S_P + q;
+    f64x4 c{0, 0, 0, 0}, d{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * a + 4 * i + q, col = 16 * b + i16;
-                const double v = c[i] + d[i];
-                if (a != b || row <= col) {                  // one value for both places, bit for bit
-                    f(row, col, v);
-                    if (row != col) f(col, row, v);
-                }
-            }
+    for (int s = 0; s < 4 * NT; s += 2) {
+        c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * s], y[4 * s], c, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * s + 4], y[4 * s + 4], d, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 16 * a + 4 * i + q, col = 16 * b + i16;
+        const double v = c[i] + d[i];
+        if (a != b || row <= col) {                          // one value for both places, bit for bit
+            f(row, col, v);
+            if (row != col) f(col, row, v);
         }
+    }
+}
+constexpr int SMALL_THREADS = 640;                           // ten tiles of 16 x 16
+
+// A in LDS (its trace in `tr`) -> P with O = P G
+template <int NT>
+__device__ __forceinline__ void small_steps(double* A, double* Q, double*& P, double* W, double inv, int steps) {
+    for (int step = 0; step < steps; ++step) {
+        sym_product<NT>(A, A, [&](int i, int j, double v) {
+            const double w = QB * A[i * S_P + j] + QC * v + (i == j ? QA : 0.0);
+            Q[i * S_P + j] = w;
+            if (step == 0) P[i * S_P + j] = w * inv;
+        });
+        __syncthreads();
+        if (step) {
+            sym_product<NT>(Q, P, [&](int i, int j, double v) { W[i * S_P + j] = v; });
+            __syncthreads();
+            double* t = P;
+            P = W;
+            W = t;
+        }
+        if (step + 1 < steps) {
+            sym_product<NT>(Q, A, [&](int i, int j, double v) { W[i * S_P + j] = v; });
+            __syncthreads();
+            sym_product<NT>(W, Q, [&](int i, int j, double v) { A[i * S_P + j] = v; });
+            __syncthreads();
+        }
+    }
 }
 
-__global__ __launch_bounds__(512) void ns_small_kernel(const SmallArgs p) {
+__global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const SmallArgs p) {
     extern __shared__ __attribute__((aligned(16))) double lds[];
     __shared__ double norm_s;
     int local;
@@ -172,104 +227,98 @@ __global__ __launch_bounds__(512) void ns_small_kernel(const SmallArgs p) {
     double *A = lds, *Q = lds + 64 * S_P, *P = lds + 2 * 64 * S_P, *W = lds + 3 * 64 * S_P;
     const double* slab = p.ws + it.slab + (size_t)local * it.chunks * 2560;
     // join the chunks in order: element e of tile t is row 16 a + 4 (e / 64) + (e % 64) / 16, column 16 b + e % 16
-    for (int e = tid; e < 2560; e += 512) {
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 8
+    for (int c = 0; c < it.chunks; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += slab[(size_t)c * 2560 + tid + SMALL_THREADS * j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = tid + SMALL_THREADS * j;
         const int t = e >> 8, a = t < 4 ? 0 : t < 7 ? 1 : t < 9 ? 2 : 3, b = t < 4 ? t : t < 7 ? t - 3 : t < 9 ? t - 5 : 3;
         const int row = 16 * a + 4 * ((e & 255) >> 6) + ((e & 63) >> 4), col = 16 * b + (e & 15);
         if (b >= nt || (a == b && row > col)) continue;
-        double v = 0.0;
-        for (int c = 0; c < it.chunks; ++c) v += slab[(size_t)c * 2560 + e];
-        A[row * S_P + col] = v;
-        A[col * S_P + row] = v;
+        A[row * S_P + col] = v[j];
+        A[col * S_P + row] = v[j];
     }
     __syncthreads();
-    if (tid == 0) {
-        double tr = 0.0;
-        for (int i = 0; i < r; ++i) tr += A[i * S_P + i];
-        norm_s = 1.0 / (sqrt(tr) + (double)p.eps);
+    if (tid < 64) {                                          // the trace is the squared norm
+        double tr = tid < R ? A[tid * S_P + tid] : 0.0;
+        for (int o = 1; o < 64; o <<= 1) tr += __shfl_xor(tr, o, 64);
+        if (tid == 0) norm_s = 1.0 / (sqrt(tr) + (double)p.eps);
     }
     __syncthreads();
     const double inv = norm_s;
-    for (int e = tid; e < R * R; e += 512) A[e / R * S_P + e % R] *= inv * inv;
+    for (int e = tid; e < 64 * R; e += SMALL_THREADS) A[(e >> 6) * S_P + (e & 63)] *= inv * inv;
     __syncthreads();
-    if (!p.steps)
-        for (int e = tid; e < R * R; e += 512) P[e / R * S_P + e % R] = e / R == e % R ? inv : 0.0;
-    for (int step = 0; step < p.steps; ++step) {
-        sym_product(A, A, nt, [&](int i, int j, double v) {
-            const double w = QB * A[i * S_P + j] + QC * v + (i == j ? QA : 0.0);
-            Q[i * S_P + j] = w;
-            if (step == 0) P[i * S_P + j] = w * inv;
-        });
-        __syncthreads();
-        const bool last = step + 1 == p.steps;
-        if (step) {
-            sym_product(Q, P, nt, [&](int i, int j, double v) { W[i * S_P + j] = v; });
-            __syncthreads();
-            double* t = P;
-            P = W;
-            W = t;
-        }
-        if (!last) {
-            sym_product(Q, A, nt, [&](int i, int j, double v) { W[i * S_P + j] = v; });
-            __syncthreads();
-            sym_product(W, Q, nt, [&](int i, int j, double v) { A[i * S_P + j] = v; });
-            __syncthreads();
-        }
-    }
-    __syncthreads();
+    if (nt == 1) small_steps<1>(A, Q, P, W, inv, p.steps);
+    else if (nt == 2) small_steps<2>(A, Q, P, W, inv, p.steps);
+    else if (nt == 3) small_steps<3>(A, Q, P, W, inv, p.steps);
+    else small_steps<4>(A, Q, P, W, inv, p.steps);
     double* out = p.ws + it.p + (size_t)local * 4096;
-    for (int e = tid; e < R * R; e += 512) out[(e / R) * 64 + e % R] = P[e / R * S_P + e % R];
+    for (int e = tid; e < 64 * R; e += SMALL_THREADS)
+        if ((e & 63) < R) out[e] = P[(e >> 6) * S_P + (e & 63)];
 }
 
 // O = P U: 16 columns of the long side a wave
 template <typename T>
 __global__ __launch_bounds__(256) void ns_apply_kernel(const SmallArgs p) {
     __shared__ double P[64 * S_P];
-    const int z = blockIdx.x / p.max_chunks, chunk = blockIdx.x % p.max_chunks;
+    const int z = blockIdx.x / p.max_parts, part = blockIdx.x % p.max_parts;
     int local;
     const SmallItem& it = find(p, z, local);
-    if (chunk >= it.chunks) return;
     const bool tall = it.m > it.n;
     const int r = tall ? it.n : it.m, l = tall ? it.m : it.n, nt = (r + 15) / 16, R = 16 * nt;
+    if (part * 64 >= l) return;
     const Io io = shifted(it.io, (size_t)local * it.m * it.n, sizeof(T));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
     const double* src = p.ws + it.p + (size_t)local * 4096;
-    for (int e = threadIdx.x; e < R * R; e += 256) P[e / R * S_P + e % R] = src[(e / R) * 64 + e % R];
+    const int c0 = part * 64 + 16 * wave, col = c0 + i16;
+    // the column's elements j = 16 t + 4 q + s for step (t, s), and what the result is added to
+    float u[4][4], old[4][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int j = 16 * t + 4 * q + s;
+            u[t][s] = j < r && col < l ? read_u<T>(io, tall ? (size_t)col * it.n + j : (size_t)j * it.n + col, false) : 0.f;
+        }
+    // element (a, i) of the result: rows are the short side, or the long one where it is the matrix's rows
+    auto place = [&](int a, int i, size_t& at) {
+        const int rr = 4 * i + q, srt = 16 * a + (tall ? i16 : rr), lng = c0 + (tall ? rr : i16);
+        at = tall ? (size_t)lng * it.n + srt : (size_t)srt * it.n + lng;
+        return srt < r && lng < l;
+    };
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            size_t at;
+            old[a][i] = place(a, i, at) && io.param ? io.param[at] : 0.f;
+        }
+    for (int e = threadIdx.x; e < 64 * R; e += 256)
+        if ((e & 63) < R) P[(e >> 6) * S_P + (e & 63)] = src[e];
     __syncthreads();
-    const int c1 = min(l, (chunk + 1) * it.width);
-    for (int c0 = chunk * it.width + 16 * wave; c0 < c1; c0 += 64) {
-        const int col = c0 + i16;
-        // the column's elements j = 16 t + 4 q + s for step (t, s)
-        double u[4][4];
+    if (c0 >= l) return;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        if (a >= nt) break;
+        f64x4 acc{0, 0, 0, 0};
 #pragma unroll
         for (int t = 0; t < 4; ++t)
+            if (t < nt)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int j = 16 * t + 4 * q + s;
-                u[t][s] = j < r && col < c1
-                              ? (double)read_u<T>(io, tall ? (size_t)col * it.n + j : (size_t)j * it.n + col, false)
-                              : 0.0;
-            }
+                for (int s = 0; s < 4; ++s) {
+                    const double pv = P[(16 * a + i16) * S_P + 16 * t + 4 * q + s];
+                    acc = tall ? __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[t][s], pv, acc, 0, 0, 0)
+                               : __builtin_amdgcn_mfma_f64_16x16x4f64(pv, (double)u[t][s], acc, 0, 0, 0);
+                }
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            if (a >= nt) break;
-            f64x4 acc{0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t < nt)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) {
-                        const double pv = P[(16 * a + i16) * S_P + 16 * t + 4 * q + s];
-                        // rows of the result: the short side, or the long one where it is the matrix's rows
-                        acc = tall ? __builtin_amdgcn_mfma_f64_16x16x4f64(u[t][s], pv, acc, 0, 0, 0)
-                                   : __builtin_amdgcn_mfma_f64_16x16x4f64(pv, u[t][s], acc, 0, 0, 0);
-                    }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int rr = 4 * i + q;
-                const int srt = 16 * a + (tall ? i16 : rr), lng = c0 + (tall ? rr : i16);
-                if (srt < r && lng < c1)
-                    write_o<T>(io, tall ? (size_t)lng * it.n + srt : (size_t)srt * it.n + lng, (float)acc[i]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            size_t at;
+            if (!place(a, i, at)) continue;
+            if (io.param) io.param[at] = old[a][i] * io.keep - io.step * (float)acc[i];
+            else ((T*)io.out)[at] = (T)(float)acc[i];        // the result's only rounding to fewer bits
         }
     }
 }
@@ -787,30 +836,37 @@ bool small(int m, int n) { return (m < n ? m : n) <= 64; }
 
 struct Group {
     int begin, end;                        // items (indices into the list of small ones)
-    int total, max_chunks;
+    int total, max_chunks, max_parts;
     size_t doubles;
 };
 // small items in groups of one launch each; the workspace is used again by every group
-int small_groups(const step_ns_item* items, const std::vector<int>& idx, std::vector<Group>& groups, std::vector<SmallItem>& out) {
+int small_groups(const step_ns_item* items, const std::vector<int>& idx, std::vector<Group>& groups, std::vector<SmallItem>& out, std::vector<int>& firsts) {
     for (size_t i = 0; i < idx.size();) {
-        Group g{(int)i, (int)i, 0, 1, 0};
+        Group g{(int)i, (int)i, 0, 1, 1, 0};
         int total = 0;
         size_t end = i;
-        while (end < idx.size() && end - i < (size_t)S_ITEMS) total += items[idx[end++]].batch;
+        long long parts = 1;
+        while (end < idx.size() && end - i < (size_t)S_ITEMS) {      // (a launch has fewer than 2^31 blocks)
+            const step_ns_item& it = items[idx[end]];
+            const long long mine = step::ceil_div(it.m > it.n ? it.m : it.n, 64), most = mine > parts ? mine : parts;
+            if (end > i && (total + it.batch) * most >= 1LL << 31) break;
+            parts = most;
+            total += items[idx[end++]].batch;
+        }
         const int share = total < 1024 ? 1024 / total : 1;
         int first = 0;
         size_t at = 0;
         for (; i < end; ++i) {
             const step_ns_item& it = items[idx[i]];
             const int l = it.m > it.n ? it.m : it.n;
-            int chunks = step::ceil_div(l, 64);
+            int chunks = step::ceil_div(l, 16 * GRAM_WAVES);
             if (chunks > share) chunks = share;
             if (chunks > 32) chunks = 32;
             SmallItem s{};
             s.m = it.m;
             s.n = it.n;
-            s.first = first;
-            s.width = step::round_up(step::ceil_div(l, chunks), 64);
+            firsts.push_back(first);
+            s.width = step::round_up(step::ceil_div(l, chunks), 16);
             s.chunks = step::ceil_div(l, s.width);
             s.slab = at;
             at += (size_t)it.batch * s.chunks * 2560;
@@ -818,6 +874,7 @@ int small_groups(const step_ns_item* items, const std::vector<int>& idx, std::ve
             at += (size_t)it.batch * 4096;
             first += it.batch;
             if (s.chunks > g.max_chunks) g.max_chunks = s.chunks;
+            if (step::ceil_div(l, 64) > g.max_parts) g.max_parts = step::ceil_div(l, 64);
             out.push_back(s);
         }
         g.end = (int)end;
@@ -837,6 +894,8 @@ int check(const step_ns_item* items, int count) {
         STEP_REQUIRE(it.m <= (1 << 21) && it.n <= (1 << 21), "step_newton_schulz: item %d: %d x %d is over 2^21 a side", i, it.m, it.n);
         STEP_REQUIRE((it.m < it.n ? it.m : it.n) <= 32768, "step_newton_schulz: item %d: %d x %d is over 32768 on both sides", i, it.m, it.n);
         total += it.batch;
+        STEP_REQUIRE((long long)it.batch * step::ceil_div(it.m > it.n ? it.m : it.n, 64) < 1LL << 31, "step_newton_schulz: item %d: %d matrices of %d x %d", i,
+                     it.batch, it.m, it.n);
     }
     STEP_REQUIRE(total <= 1 << 24, "step_newton_schulz: %lld matrices", total);
     return STEP_OK;
@@ -909,7 +968,8 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
     if (!idx.empty()) {
         std::vector<Group> groups;
         std::vector<SmallItem> sm;
-        small_groups(items, idx, groups, sm);
+        std::vector<int> firsts;
+        small_groups(items, idx, groups, sm, firsts);
         constexpr size_t lds = 4 * 64 * S_P * sizeof(double);
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ns_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) {
@@ -922,15 +982,17 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
             a.total = g.total;
             a.steps = steps;
             a.max_chunks = g.max_chunks;
+            a.max_parts = g.max_parts;
             a.eps = eps;
             a.ws = (double*)ws;
+            for (int i = 0; i < S_ITEMS; ++i) a.first[i] = i < a.items ? firsts[g.begin + i] : 0x7fffffff;
             for (int i = 0; i < a.items; ++i) {
                 a.item[i] = sm[g.begin + i];
                 a.item[i].io = io_of(items[idx[g.begin + i]]);
             }
-            hipLaunchKernelGGL(ns_gram_kernel<T>, dim3((unsigned)g.total * g.max_chunks), dim3(256), 0, st, a);
-            hipLaunchKernelGGL(ns_small_kernel, dim3((unsigned)g.total), dim3(512), lds, st, a);
-            hipLaunchKernelGGL(ns_apply_kernel<T>, dim3((unsigned)g.total * g.max_chunks), dim3(256), 0, st, a);
+            hipLaunchKernelGGL(ns_gram_kernel<T>, dim3((unsigned)g.total * g.max_chunks), dim3(64 * GRAM_WAVES), 0, st, a);
+            hipLaunchKernelGGL(ns_small_kernel, dim3((unsigned)g.total), dim3(SMALL_THREADS), lds, st, a);
+            hipLaunchKernelGGL(ns_apply_kernel<T>, dim3((unsigned)g.total * g.max_parts), dim3(256), 0, st, a);
         }
     }
     for (int i = 0; i < count; ++i) {
@@ -959,7 +1021,8 @@ extern "C" size_t step_newton_schulz_ws_bytes(const step_ns_item* items, int cou
         }
         std::vector<Group> groups;
         std::vector<SmallItem> sm;
-        small_groups(items, idx, groups, sm);
+        std::vector<int> firsts;
+        small_groups(items, idx, groups, sm, firsts);
         for (const Group& g : groups)
             if (g.doubles * sizeof(double) > most) most = g.doubles * sizeof(double);
         return most;
