@@ -4,6 +4,7 @@ There is NO fallback: if the shared library is missing or a call fails, this rai
 Tensors are passed as raw device pointers; the launch stream is torch's current stream.
 """
 import ctypes
+import functools
 import os
 
 import torch
@@ -169,7 +170,7 @@ def call(name, *args):
         else:
             conv.append(a)
     fn = getattr(lib, name)
-    current = torch.cuda.current_device()
+    current = torch._C._cuda_getDevice()
     if index < 0 or index == current:
         rc = fn(*conv, torch._C._cuda_getCurrentRawStream(current))
     else:
@@ -182,3 +183,18 @@ def call(name, *args):
 def query(name, *args):
     """Call a size_t-returning helper."""
     return getattr(load(), name)(*args)
+
+
+@functools.lru_cache(maxsize=4096)
+def size(name, *shape):
+    """query() for helpers that depend on whole numbers alone, asked once for each"""
+    return query(name, *shape)
+
+
+def differentiable_once(backward):
+    """torch's once_differentiable, at no cost where no second derivative is prepared"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run

@@ -326,8 +326,8 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const SmallArgs p) {
 // ---------------------------------------------------------------------------------------------- r > 64
 constexpr int TN = 128, KS = 32;                  // columns of an output tile, contraction per stage
 constexpr int ROWB = 128;                         // bytes of a row's stage: 32 hi, 32 lo
-constexpr int EP = TN + 4;                        // pitch of a tile in LDS at the end
-constexpr float SX = 16384.f, SA = 16384.f, SB = 8192.f;   // scales of X, A and q(A): elements under 1.21, 1.47, 3.45
+// scales of X, of A and q(A) A, and of products of one, two and three q(A): elements under 1.21, 1.47, 3.45, 11.9 and 41
+constexpr float SX = 16384.f, SA = 16384.f, SQ[3] = {8192.f, 4096.f, 1024.f};
 constexpr int CUS = 256;
 constexpr int NORM_BLOCKS = 1024;
 
@@ -336,7 +336,10 @@ struct Big {
     int m, n, r, l, R, L, RA;                     // R, L: r and l rounded up to whole tiles; RA: rows that X and A have
     float eps;
     double* part;                                 // [batch][NORM_BLOCKS] sums of squares
-    char *x, *xt, *xt2, *a, *b;                   // packed matrices, one after the other for the batch
+    char *x, *xt, *xt2;                           // packed matrices, one after the other for the batch
+    const char *s1, *s2;                          // R x R (RA rows) operands of a product, and its result
+    char* s3;
+    float scale;                                  // result's scale over the operands'
     float* slab;                                  // shares of split tiles
 };
 
@@ -347,13 +350,16 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const Big p) {
     const Io io = shifted(p.io, e * blockIdx.y, sizeof(T));
     double s = 0.0;
     constexpr int N = 16 / (int)sizeof(T);
-    if (!io.momentum && ((uintptr_t)io.g & 15) == 0) {
+    if (!io.momentum) {
         const size_t packs = e / N;
+        double part[4] = {0.0, 0.0, 0.0, 0.0};               // four chains
+#pragma unroll 2
         for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (size_t)gridDim.x * 256) {
-            const Pack<T, N> q = ((const Pack<T, N>*)io.g)[i];
+            const Pack<T, N> q = load_pack<T, N>((const T*)io.g + i * N);
 #pragma unroll
-            for (int k = 0; k < N; ++k) s += (double)(float)q.v[k] * (double)(float)q.v[k];
+            for (int k = 0; k < N; ++k) part[k & 3] += (double)(float)q.v[k] * (double)(float)q.v[k];
         }
+        s = (part[0] + part[1]) + (part[2] + part[3]);
         if (blockIdx.x == 0 && threadIdx.x < (unsigned)(e - packs * N)) {
             const double v = (double)(float)((const T*)io.g)[packs * N + threadIdx.x];
             s += v * v;
@@ -388,8 +394,8 @@ __device__ __forceinline__ void put8(char* to, const float* v) {
     *(f16x8*)(to + 64) = lo;
 }
 
-// X_0 scaled and packed, both ways: one 64 x 64 tile a block.  Rows behind R (X has RA) become zero; A's become so too: the
-// products read them, whose results are not written.
+// X_0 scaled and packed, both ways: one 64 x 64 tile a block.  (Rows behind R, which X and the R x R matrices have up to RA, are
+// read by the products whose results are not written: they stay as they are.)
 template <typename T>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     __shared__ float sm[64][65];
@@ -419,10 +425,6 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sm[a][b + e];
         put8(packed(x, i0 + a, k0 + b, p.L), v);
-        if (i0 >= p.R) {
-            if (k0 + b < p.R) put8(packed(p.a + (size_t)z * p.RA * p.R * 4, i0 + a, k0 + b, p.R), v);
-            continue;
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = sm[b + e][a];
         put8(packed(xt, k0 + a, i0 + b, p.R), v);
@@ -455,6 +457,10 @@ __device__ __forceinline__ void multiply(Acc<MT>& acc, const Frag<MT>& f) {
         for (int b = 0; b < 2; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bl[b], acc.w[a][b], 0, 0, 0);
 }
 
+template <int MT>
+constexpr int stages_of() {
+    return MT == 4 ? 3 : 4;
+}
 // acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 128) of B over the stages [s0, s1): operands packed alike, K along both.
 // A stage lies in LDS as rows of 128 bytes whose eight 16-byte pieces are in the order piece ^ order(row): 16 neighbouring rows
 // are read from different banks (64 banks hold two rows).  Three stages in LDS, copied there directly, two of them in flight.  A wave reads the
@@ -464,7 +470,7 @@ __device__ __forceinline__ void multiply(Acc<MT>& acc, const Frag<MT>& f) {
 // bytes a cycle); 64 x 64 a wave needs 125.
 template <int MT>
 __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
-    constexpr int TM = 64 * MT, STAGE = (TM + TN) * ROWB, NA = TM / 32, NL = NA + 4;      // copies of a wave: NA + 4 of 8 rows
+    constexpr int TM = 64 * MT, STAGE = (TM + TN) * ROWB, NST = stages_of<MT>(), NA = TM / 32, NL = NA + 4;      // copies of a wave: NA + 4 of 8 rows
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, q = lane >> 5;
     const size_t pitch = (size_t)(K / KS) * ROWB;
     const int lrow = lane >> 3, piece = (lane & 7) ^ lrow, order = (l31 & 7) ^ ((l31 >> 3) & 1);
@@ -501,16 +507,15 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
             f.bl[t] = *(const f16x8*)(rb + lo + t * 32 * ROWB);
         }
     };
-    issue(s0, 0);
-    issue(s0 + 1, 1);
-    issue(s0 + 2, 2);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+#pragma unroll
+    for (int i = 0; i < NST; ++i) issue(s0 + i, i);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * NL) : "memory");
     __builtin_amdgcn_s_barrier();
     Frag<MT> f0, f1;
     read(f0, 0, 0);
     int buf = 0;
     for (int s = s0; s < s1; ++s) {
-        const int next = buf == 2 ? 0 : buf + 1;
+        const int next = buf == NST - 1 ? 0 : buf + 1;
         __builtin_amdgcn_s_waitcnt(0xc07f);       // lgkmcnt(0): f0, read half a stage ago.  (The builtin, which the compiler counts
         __builtin_amdgcn_sched_barrier(0);        // too: else it waits for f1 as well before f0 is used.)
         read(f1, buf, 1);
@@ -522,12 +527,13 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
         }
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070 | NL);  // lgkmcnt(0), vmcnt(NL): f1, and this wave's copies of the next stage
+        constexpr int FLY = (NST - 2) * NL;       // lgkmcnt(0), vmcnt(FLY): f1, and this wave's copies of the next stage
+        __builtin_amdgcn_s_waitcnt(0x0070 | (FLY & 15) | FLY >> 4 << 14);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         read(f0, next, 0);
-        issue(s + 3, buf);
+        issue(s + NST, buf);
         multiply(acc, f1);
 #pragma unroll
         for (int i = 0; i < 2 * MT + 4; ++i) {
@@ -561,7 +567,7 @@ __device__ __forceinline__ void each(const Acc<MT>& acc, F f) {
 }
 
 // The products: what they multiply, and what becomes of `rows` rows of a tile [rows][EP] in LDS that begins at (i0, j0).
-enum Product { XXT, POLY, UPDATE, RESULT };
+enum Product { XXT, POLY, SYM, UPDATE, RESULT };                             // X X^T; q(s1); s1 s2, commuting; s2 X; s2 X as the result
 
 // tiles of 64 MT x 128 that hold the diagonal of an R x R matrix and what is over it, in blocks of 1024 x 1024 (which share
 // their operands in an XCD's L2): block column after block column
@@ -608,7 +614,7 @@ template <int PROD, int MT>
 __device__ __forceinline__ void locate(const Big& p, int tile, int& z, int& i0, int& j0, int tiles) {
     z = tile / tiles;
     int t = tile - z * tiles, ti, tj;
-    if constexpr (PROD == XXT || PROD == POLY) {
+    if constexpr (PROD <= SYM) {
         tri_tile<MT>(t, p.R / TN, ti, tj);
     } else {                                       // eight columns of tiles at a time
         const int rows = p.L / (64 * MT), cols = p.R / TN, g = t / (8 * rows), w = cols - 8 * g < 8 ? cols - 8 * g : 8, in = t - g * 8 * rows;
@@ -618,14 +624,14 @@ __device__ __forceinline__ void locate(const Big& p, int tile, int& z, int& i0, 
     i0 = ti * 64 * MT;
     j0 = tj * TN;
 }
+// pitch of a tile in LDS at the end: rows of 16-byte pieces, or columns in different banks where the result is written by columns
 template <int PROD>
-__device__ __forceinline__ float scale_of() {
-    return PROD == XXT ? SA / (SX * SX) : PROD == POLY ? (float)QC * SB / (SA * SA) : PROD == UPDATE ? SX / (SB * SX) : 1.f / (SB * SX);
+constexpr int pitch_of() {
+    return PROD == RESULT ? TN + 1 : TN + 4;
 }
-
 // columns of ROWS rows in LDS as rows of a packed matrix: four neighbouring threads write 64 bytes of a row, and a wave reads at
 // most two values from a bank
-template <int ROWS, typename F>
+template <int ROWS, int EP, typename F>
 __device__ __forceinline__ void transposed(const float* sm, F to) {
 #pragma unroll 4
     for (int u = threadIdx.x; u < ROWS * 16; u += 256) {
@@ -642,10 +648,11 @@ __device__ __forceinline__ void transposed(const float* sm, F to) {
 template <int PROD, int ROWS, typename T>
 __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, int j0) {
     constexpr int N = ROWS == 8 ? 1 : ROWS * 16 / 256, M = N < 8 ? N : 8;     // eight neighbours N times a thread, M of them at a time
+    constexpr int EP = pitch_of<PROD>();
     const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 8;
-    if constexpr (PROD == XXT || PROD == POLY) {
-        char* a = p.a + (size_t)z * p.RA * p.R * 4;
-        char* to = PROD == XXT ? a : p.b + (size_t)z * p.R * p.R * 4;
+    if constexpr (PROD <= SYM) {
+        char* to = p.s3 + (size_t)z * p.RA * p.R * 4;
+        const char* a = p.s1 + (size_t)z * p.RA * p.R * 4;
         const int cb = j0 / TN;
         for (int u = 0; u < N; u += M) {
             f16x8 hi[M], lo[M];
@@ -654,7 +661,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
                 for (int k = 0; k < M; ++k) {
                     const int i = row + 16 * (u + k);
                     if (i >= ROWS || (i0 + i) / TN > cb) continue;
-                    const char* s = packed(a, i0 + i, j0 + col, p.R);
+                    const char* s = packed((char*)a, i0 + i, j0 + col, p.R);
                     hi[k] = *(const f16x8*)s;
                     lo[k] = *(const f16x8*)(s + 64);
                 }
@@ -668,8 +675,8 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
                 for (int e = 0; e < 8; ++e) {
                     v[e] = sm[i * EP + col + e];
                     if constexpr (PROD == POLY) {
-                        v[e] += (float)QB * (SB / SA) * ((float)hi[k][e] + (float)lo[k][e]);
-                        if (i0 + i == j0 + col + e) v[e] += (float)QA * SB;
+                        v[e] += (float)QB * (SQ[0] / SA) * ((float)hi[k][e] + (float)lo[k][e]);
+                        if (i0 + i == j0 + col + e) v[e] += (float)QA * SQ[0];
                         sm[i * EP + col + e] = v[e];
                     }
                 }
@@ -677,7 +684,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
             }
         }
         if constexpr (PROD == POLY) __syncthreads();
-        transposed<ROWS>(sm, [&](int i, int j) { return (i0 + i) / TN >= cb ? nullptr : packed(to, j0 + j, i0 + i, p.R); });
+        transposed<ROWS, EP>(sm, [&](int i, int j) { return (i0 + i) / TN >= cb ? nullptr : packed(to, j0 + j, i0 + i, p.R); });
     } else if constexpr (PROD == UPDATE) {                                   // rows: the long side
         char* xt = p.xt2 + (size_t)z * p.R * p.L * 4;
         char* x = p.x + (size_t)z * p.RA * p.L * 4;
@@ -688,15 +695,36 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
             for (int e = 0; e < 8; ++e) v[e] = sm[i * EP + col + e];
             put8(packed(xt, i0 + i, j0 + col, p.R), v);
         }
-        transposed<ROWS>(sm, [&](int i, int j) { return packed(x, j0 + j, i0 + i, p.L); });
+        transposed<ROWS, EP>(sm, [&](int i, int j) { return packed(x, j0 + j, i0 + i, p.L); });
     } else {
+        // packs along the matrix's rows: of the tile's columns where the long side is the matrix's rows, of its rows otherwise
         const Io io = shifted(p.io, (size_t)p.m * p.n * z, sizeof(T));
         const bool tall = p.m > p.n;
-#pragma unroll 4
-        for (int u = threadIdx.x; u < ROWS * TN; u += 256) {
-            const int i = tall ? u / TN : u % ROWS, j = tall ? u % TN : u / ROWS;
-            if (i0 + i < p.l && j0 + j < p.r)
-                write_o<T>(io, tall ? (size_t)(i0 + i) * p.n + j0 + j : (size_t)(j0 + j) * p.n + i0 + i, sm[i * EP + j]);
+        constexpr int V = 16 / (int)sizeof(T), RP = ROWS / V;
+#pragma unroll 2
+        for (int u = threadIdx.x; u < ROWS * TN / V; u += 256) {
+            const int i = tall ? u / (TN / V) : u % RP * V, j = tall ? u % (TN / V) * V : u / RP;
+            const int left = tall ? (i0 + i < p.l ? p.r - (j0 + j) : 0) : (j0 + j < p.r ? p.l - (i0 + i) : 0);
+            if (left <= 0) continue;
+            const size_t at = tall ? (size_t)(i0 + i) * p.n + j0 + j : (size_t)(j0 + j) * p.n + i0 + i;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = tall ? sm[i * EP + j + e] : sm[(i + e) * EP + j];
+            if (left >= V && !io.param) {
+                Pack<T, V> o;
+#pragma unroll
+                for (int e = 0; e < V; ++e) o.v[e] = (T)v[e];                // the result's only rounding to fewer bits
+                store_pack<T, V>((T*)io.out + at, o);
+            } else if (left >= V) {
+                Pack<float, V> o = load_pack<float, V>(io.param + at);
+#pragma unroll
+                for (int e = 0; e < V; ++e) o.v[e] = o.v[e] * io.keep - io.step * v[e];
+                store_pack<float, V>(io.param + at, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (e < left) write_o<T>(io, at + e, v[e]);
+            }
         }
     }
 }
@@ -720,12 +748,13 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
     if constexpr (PROD == XXT) {
         A = B = p.x + (size_t)z * p.RA * p.L * 4;
         K = p.L;
-    } else if constexpr (PROD == POLY) {
-        A = B = p.a + (size_t)z * p.RA * p.R * 4;
+    } else if constexpr (PROD <= SYM) {
+        A = p.s1 + (size_t)z * p.RA * p.R * 4;
+        B = PROD == POLY ? A : p.s2 + (size_t)z * p.RA * p.R * 4;
         K = p.R;
     } else {
         A = p.xt + (size_t)z * p.R * p.L * 4;
-        B = p.b + (size_t)z * p.R * p.R * 4;
+        B = p.s2 + (size_t)z * p.RA * p.R * 4;
         K = p.R;
     }
     const int stages = K / KS;
@@ -738,10 +767,10 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[a][b][e] = acc.w[a][b][e] = 0.f;
     main_loop(acc, A, B, K, i0, j0, s0, s1, smem);
-    const float f = scale_of<PROD>();
+    const float f = p.scale;
     if (whole) {
         float* sm = (float*)smem;
-        each(acc, [&](int i, int j, float v) { sm[i * EP + j] = v * f; });
+        each(acc, [&](int i, int j, float v) { sm[i * pitch_of<PROD>() + j] = v * f; });
         __syncthreads();
         finish<PROD, 64 * MT, T>(p, sm, z, i0, j0);
     } else {
@@ -752,6 +781,7 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
 // eight rows of a split tile, its shares added in order
 template <int PROD, int MT, typename T>
 __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, int full, int splits) {
+    constexpr int EP = pitch_of<PROD>();
     __shared__ __attribute__((aligned(16))) float sm[8 * EP];
     int z, i0, j0;
     locate<PROD, MT>(p, full + blockIdx.x, z, i0, j0, tiles);
@@ -760,42 +790,54 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, in
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) v += *(const f32x4*)(slab + (size_t)s * 64 * MT * TN);
-    *(f32x4*)(sm + i * EP + j) = v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sm[i * EP + j + e] = v[e];
     __syncthreads();
     finish<PROD, 8, T>(p, sm, z, i0 + blockIdx.y * 8, j0);
 }
 
 // ---------------------------------------------------------------------------------------------- host
+// How a product's tiles are shared out: `mt` 32-row tiles a wave; whole rounds over the CUs, and the rest in `splits` parts
 struct Share {
-    int full, rest, splits;
+    int mt, tiles, full, rest, splits;
 };
-// `total` tiles of `stages` stages over the CUs: whole rounds, and the rest in parts of 8 stages at least
-Share share(long long total, int stages) {
-    Share s{(int)(total / CUS * CUS), (int)(total % CUS), 1};
-    if (s.rest) {
-        s.splits = CUS / s.rest;
-        if (s.splits > stages / 8) s.splits = stages / 8;
-        if (s.splits > 48) s.splits = 48;
-        if (s.splits < 2) s.splits = 1;
-    }
+// The variant that takes the least time by this count, in cycles: a stage takes 1536 on the matrix cores at 256 x 128 a tile, half of it
+// at 128 x 128 (1600 and 850 were measured, with the waits); a tile's beginning and end 8000; writing and joining the parts
+// of split tiles 26000 (9 us over 16 tiles, 14 us over 75).  4096 x 4096: 272 tiles of 256 x 128 as 256 and 16 x 16 parts;
+// three stacked 1152 x 1152: 135 tiles of 128 x 128 at once (19 us) and not 75 x 3 parts of 256 x 128 (26 + 12 us).
+Share share(int mt, long long tiles, long long total) {
+    Share s{mt, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
     return s;
 }
+double cycles(const Share& s, int stages) {
+    const double one = s.mt == 4 ? 1600 : 850, round = stages * one + 8000;
+    return s.full / CUS * round + (s.rest ? (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + 8000 + 26000 : round) : 0);
+}
+Share best(const Share& a, const Share& b, int stages) { return cycles(b, stages) < cycles(a, stages) ? b : a; }
+Share fastest(int mt, long long tiles, int nb, int stages) {
+    Share s = share(mt, tiles, tiles * nb), t = s;
+    if (s.rest) {
+        t.splits = CUS / s.rest;
+        if (t.splits > stages / 4) t.splits = stages / 4;
+        if (t.splits > 48) t.splits = 48;
+        if (t.splits < 2) t.splits = 1;
+    }
+    return best(s, t, stages);
+}
 struct Layout {
-    size_t part, x, xt, xt2, a, b, slab, total;
-    int sub, mt, R, L, RA, tri, all;
-    Share xxt, poly, update;
+    size_t part, x, xt, xt2, r[4], slab, total;
+    int sub, R, L, RA, group;
+    Share xxt, sym, update;
 };
-Layout layout_of(int nb, int r, int l, int mt) {
+Layout layout_of(int nb, int r, int l) {
     Layout o{};
-    o.mt = mt;
     o.R = step::round_up(r, TN);
-    o.L = step::round_up(l, 64 * mt);
-    o.RA = step::round_up(o.R, 64 * mt);
-    o.tri = tri_tiles(o.R, mt / 2);
-    o.all = o.L / (64 * mt) * (o.R / TN);
-    o.xxt = share((long long)o.tri * nb, o.L / KS);
-    o.poly = share((long long)o.tri * nb, o.R / KS);
-    o.update = share((long long)o.all * nb, o.R / KS);
+    o.L = step::round_up(l, 256);
+    o.RA = step::round_up(r, 256);
+    const int t4 = tri_tiles(o.R, 2), t2 = tri_tiles(o.R, 1), sx = o.L / KS, sr = o.R / KS;
+    o.xxt = best(fastest(4, t4, nb, sx), fastest(2, t2, nb, sx), sx);
+    o.sym = best(fastest(4, t4, nb, sr), fastest(2, t2, nb, sr), sr);
+    o.update = best(fastest(4, (long long)(o.L / 256) * (o.R / TN), nb, sr), fastest(2, (long long)(o.L / 128) * (o.R / TN), nb, sr), sr);
     return o;
 }
 // workspace of a stack of `batch` matrices with r > 64, `sub` of them at a time
@@ -805,9 +847,7 @@ Layout layout(int batch, int m, int n) {
     const size_t fit = most / ((size_t)step::round_up(r, 256) * step::round_up(l, 256));
     int sub = (int)(fit < (size_t)batch ? fit : (size_t)batch);
     sub = sub < 1 ? 1 : sub > 1024 ? 1024 : sub;
-    // tiles of 256 rows where they fill the card, of 128 otherwise
-    Layout o = layout_of(sub, r, l, 4);
-    if ((long long)o.all * sub < CUS) o = layout_of(sub, r, l, 2);
+    Layout o = layout_of(sub, r, l);
     o.sub = sub;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -820,15 +860,16 @@ Layout layout(int batch, int m, int n) {
     o.x = take(sub * RA * L * 4);
     o.xt = take(sub * R * L * 4);
     o.xt2 = take(sub * R * L * 4);
-    o.a = take(sub * RA * R * 4);
-    o.b = take(sub * R * R * 4);
-    size_t slab = 0;
-    for (const Share& s : {o.xxt, o.poly, o.update}) {
-        // a smaller last part of the batch is shared out anew: at most 256 parts of tiles either way
-        const size_t parts = s.splits > 1 || sub < batch ? CUS : 0;
-        if (parts > slab) slab = parts;
-    }
-    o.slab = take(slab * 64 * o.mt * TN * 4);
+    // steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
+    // products of r x r matrices, of which each further step takes three more.  Worth it where X is longer than wide (by count at
+    // l > r; from l = 2 r it also outweighs that r x r products fill the card less).  An error of A grows by a^2 = 12 in each
+    // step of a group for the smallest eigenvalues: three fp32-accurate steps cost them 2e-5 of the largest, less than what
+    // X X^T over that length is off by.
+    o.group = l >= 2 * r ? 3 : 1;
+    for (int i = 0; i < (o.group > 1 ? 4 : 2); ++i) o.r[i] = take(sub * RA * R * 4);
+    // shares of split tiles: fewer than one a CU, of 256 x 128 at most.  A last part of the batch that is smaller is shared out anew.
+    const bool any = sub < batch || o.xxt.splits > 1 || o.sym.splits > 1 || o.update.splits > 1;
+    o.slab = take(any ? (size_t)CUS * 256 * TN * 4 : 0);
     o.total = at;
     return o;
 }
@@ -902,19 +943,23 @@ int check(const step_ns_item* items, int count) {
 }
 
 template <int PROD, int MT, typename T>
-int product(const Big& p, int tiles, const Share& s, hipStream_t st) {
+int product_of(const Big& p, const Share& s, hipStream_t st) {
     auto kern = ns_product_kernel<PROD, MT, T>;
-    constexpr size_t lds = 3 * (64 * MT + TN) * ROWB;
+    constexpr size_t lds = stages_of<MT>() * (64 * MT + TN) * ROWB;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
         return STEP_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL(kern, dim3(s.full + s.rest * s.splits), dim3(256), lds, st, p, tiles, s.full, s.splits);
-    if (s.splits > 1) hipLaunchKernelGGL((ns_join_kernel<PROD, MT, T>), dim3(s.rest, 8 * MT), dim3(256), 0, st, p, tiles, s.full, s.splits);
+    hipLaunchKernelGGL(kern, dim3(s.full + s.rest * s.splits), dim3(256), lds, st, p, s.tiles, s.full, s.splits);
+    if (s.splits > 1) hipLaunchKernelGGL((ns_join_kernel<PROD, MT, T>), dim3(s.rest, 8 * MT), dim3(256), 0, st, p, s.tiles, s.full, s.splits);
     return STEP_OK;
 }
-template <typename T, int MT>
+template <int PROD, typename T>
+int product(const Big& p, const Share& s, hipStream_t st) {
+    return s.mt == 4 ? product_of<PROD, 4, T>(p, s, st) : product_of<PROD, 2, T>(p, s, st);
+}
+template <typename T>
 int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
     const Layout all = layout(it.batch, it.m, it.n);
     Big p{};
@@ -929,11 +974,11 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
     p.part = (double*)(base + all.part);
     p.slab = (float*)(base + all.slab);
     p.x = base + all.x;
-    p.a = base + all.a;
-    p.b = base + all.b;
+    char* r[4];
+    for (int i = 0; i < 4; ++i) r[i] = base + all.r[i];
     for (int b0 = 0; b0 < it.batch; b0 += all.sub) {
         const int nb = it.batch - b0 < all.sub ? it.batch - b0 : all.sub;
-        const Layout o = layout_of(nb, p.r, p.l, MT);
+        const Layout o = layout_of(nb, p.r, p.l);
         const size_t by = (size_t)b0 * it.m * it.n;
         p.io = io;
         p.io.g = (const T*)io.g + by;
@@ -943,16 +988,51 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
         p.xt = base + all.xt;
         p.xt2 = base + all.xt2;
         hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(NORM_BLOCKS, nb), dim3(256), 0, st, p);
-        hipLaunchKernelGGL(ns_pack_kernel<T>, dim3(p.L / 64, p.RA / 64, nb), dim3(256), 0, st, p);
-        for (int s = 0; s < steps; ++s) {
-            int rc = product<XXT, MT, float>(p, o.tri, o.xxt, st);
-            if (rc == STEP_OK) rc = product<POLY, MT, float>(p, o.tri, o.poly, st);
-            if (rc == STEP_OK) rc = s + 1 < steps ? product<UPDATE, MT, float>(p, o.all, o.update, st) : product<RESULT, MT, T>(p, o.all, o.update, st);
-            if (rc != STEP_OK) return rc;
+        hipLaunchKernelGGL(ns_pack_kernel<T>, dim3(p.L / 64, p.R / 64, nb), dim3(256), 0, st, p);
+        int rc = STEP_OK;
+        // s3 <- s1 s2, scales f1, f2 -> f3
+        auto sym = [&](const char* s1, float f1, const char* s2, float f2, char* s3, float f3) {
+            p.s1 = s1;
+            p.s2 = s2;
+            p.s3 = s3;
+            p.scale = f3 / (f1 * f2);
+            if (rc == STEP_OK) rc = product<SYM, float>(p, o.sym, st);
+        };
+        auto poly = [&](const char* a, char* to) {
+            p.s1 = a;
+            p.s3 = to;
+            p.scale = (float)QC * SQ[0] / (SA * SA);
+            if (rc == STEP_OK) rc = product<POLY, float>(p, o.sym, st);
+        };
+        for (int s = 0; s < steps && rc == STEP_OK;) {
+            const int g = steps - s < all.group ? steps - s : all.group;
+            char *A = r[0], *P = r[1], *Q = r[1], *W = r[2], *F = r[3];      // F: free
+            p.s3 = A;
+            p.scale = SA / (SX * SX);
+            rc = product<XXT, float>(p, o.xxt, st);
+            poly(A, Q);
+            for (int k = 1; k < g; ++k) {
+                sym(Q, SQ[0], A, SA, W, SA);                                 // A <- q(A) A q(A)
+                sym(W, SA, Q, SQ[0], A, SA);
+                if (k > 1) {                                                 // (the last q(A) is no longer needed, P is)
+                    F = Q;
+                }
+                poly(A, F);
+                Q = F;
+                sym(Q, SQ[0], P, SQ[k - 1], W, SQ[k]);
+                F = P;
+                P = W;
+                W = F;
+            }
+            p.s2 = P;
+            s += g;
+            p.scale = s < steps ? SX / (SQ[g - 1] * SX) : 1.f / (SQ[g - 1] * SX);
+            if (rc == STEP_OK) rc = s < steps ? product<UPDATE, float>(p, o.update, st) : product<RESULT, T>(p, o.update, st);
             char* t = p.xt;
             p.xt = p.xt2;
             p.xt2 = t;
         }
+        if (rc != STEP_OK) return rc;
     }
     return STEP_OK;
 }
@@ -997,8 +1077,7 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
     }
     for (int i = 0; i < count; ++i) {
         if (small(items[i].m, items[i].n)) continue;
-        const int rc = layout(items[i].batch, items[i].m, items[i].n).mt == 4 ? run_big<T, 4>(items[i], io_of(items[i]), steps, eps, (char*)ws, st)
-                                                                                : run_big<T, 2>(items[i], io_of(items[i]), steps, eps, (char*)ws, st);
+        const int rc = run_big<T>(items[i], io_of(items[i]), steps, eps, (char*)ws, st);
         if (rc != STEP_OK) return rc;
     }
     return step::check_launch("step_newton_schulz");

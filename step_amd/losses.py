@@ -74,16 +74,15 @@ class _PolicyLossFn(torch.autograd.Function):
         classes = logits.shape[-1]
         rows = logits.numel() // classes
         z = logits.contiguous()
-        dev = z.device
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        stats = torch.empty(3, dtype=torch.float32, device=dev)
-        logp = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+        loss = z.new_empty((), dtype=torch.float32)
+        stats = z.new_empty(3, dtype=torch.float32)
+        logp = z.new_empty(logits.shape[:-1], dtype=torch.float32)
         need = ctx.needs_input_grad[0]
         grad = torch.empty_like(z) if need else None
         ctx.mark_non_differentiable(logp, stats)
         ctx.config = (clip_low, clip_high, beta)
-        nb = _lib.query("step_policy_loss_ws_bytes", rows)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+        nb = _lib.size("step_policy_loss_ws_bytes", rows)
+        ws = z.new_empty(nb, dtype=torch.uint8)
         if not rows:
             loss.zero_(), stats.zero_()
         else:
@@ -95,7 +94,7 @@ class _PolicyLossFn(torch.autograd.Function):
         return loss, logp, stats
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.differentiable_once
     def backward(ctx, g, _logp, _stats):
         z, actions, old_logp, advantages, ref_logp, mask = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
@@ -132,12 +131,13 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
     if not (0.0 <= low <= 1.0 and high >= 0.0):
         raise _lib.StepHipError("policy_loss: clip (%r, %r): 0 <= low <= 1 and high >= 0 wanted" % (low, high))
     lead = logits.shape[:-1]
+    where = logits.get_device()
 
     def per_row(t, name, kinds, to):
         if not isinstance(t, torch.Tensor) or t.dtype not in kinds:
             raise _lib.StepHipError("policy_loss: %s: a tensor of %s wanted, got %s" % (
                 name, " / ".join(str(k)[6:] for k in kinds), getattr(t, "dtype", type(t).__name__)))
-        if t.device != logits.device:
+        if t.get_device() != where or t.is_meta != logits.is_meta:
             raise _lib.StepHipError("policy_loss: %s is on %s, logits on %s" % (name, t.device, logits.device))
         if t.dtype is to and t.shape == lead and not t.requires_grad and t.is_contiguous():
             return t

@@ -800,13 +800,6 @@ class BnRowsFn(torch.autograd.Function):
 
 
 # ----------------------------------------------------------------------- layer norm
-def _dtype_code(t, what):
-    code = _lib.DTYPES.get(t.dtype)
-    if code is None:
-        raise _lib.StepHipError("%s: float32, bfloat16 or float16 wanted, got %s" % (what, t.dtype))
-    return code
-
-
 class LayerNormFn(torch.autograd.Function):
     """Layer norm over the last axis; saves the rows' mean and 1 / sqrt(variance + eps) for the backward"""
 
@@ -822,7 +815,7 @@ class LayerNormFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         mean = rstd = stats = None
         if need[0] or need[1] or need[2]:
-            stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+            stats = x.new_empty((2, rows), dtype=torch.float32)
             mean = stats.data_ptr()
             rstd = mean + 4 * rows
             ctx.save_for_backward(x, w, stats)
@@ -831,22 +824,21 @@ class LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.differentiable_once
     def backward(ctx, dy):
         x, w, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         cols = x.shape[-1]
         rows = x.numel() // cols
-        dev = x.device
         dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty(cols, dtype=ctx.wtype, device=dev) if need_w else None
-        db = torch.empty(cols, dtype=ctx.wtype, device=dev) if need_b else None
+        dw = x.new_empty(cols, dtype=ctx.wtype) if need_w else None
+        db = x.new_empty(cols, dtype=ctx.wtype) if need_b else None
         if not rows:
             return dx, dw.zero_() if need_w else None, db.zero_() if need_b else None, None
         nb, ws = 0, None
         if need_w or need_b:
-            nb = _lib.query("step_layernorm_bwd_ws_bytes", rows, cols)
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+            nb = _lib.size("step_layernorm_bwd_ws_bytes", rows, cols)
+            ws = x.new_empty(nb, dtype=torch.uint8)
         mean = stats.data_ptr()
         _lib.call("step_layernorm_bwd", dy.contiguous(), x, w, mean, mean + 4 * rows, dx, dw, db, rows, cols, _lib.DTYPES[x.dtype],
                   _lib.DTYPES[ctx.wtype], ws, nb)
@@ -859,20 +851,22 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     x float32, bfloat16 or float16; weight and bias (cols,) of x's type or float32, either may be None.  Statistics and
     gradient sums are fp32, every result is rounded once.  Needs no statistics of the batch: a row's result is the same
     in any batch, on any number of ranks and for a single row."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise _lib.StepHipError("layer_norm: x %s has no last axis to normalise" % (tuple(x.shape),))
-    _dtype_code(x, "layer_norm")
-    cols = x.shape[-1]
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        raise _lib.StepHipError("layer_norm: x %s has no last axis to normalise" % (tuple(shape),))
+    if x.dtype not in _lib.DTYPES:
+        raise _lib.StepHipError("layer_norm: float32, bfloat16 or float16 wanted, got %s" % x.dtype)
+    where = x.get_device()
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if tuple(t.shape) != (cols,):
-            raise _lib.StepHipError("layer_norm: %s %s does not fit x %s" % (name, tuple(t.shape), tuple(x.shape)))
-        if t.dtype not in (x.dtype, torch.float32):
+        if t.shape != shape[-1:]:
+            raise _lib.StepHipError("layer_norm: %s %s does not fit x %s" % (name, tuple(t.shape), tuple(shape)))
+        if t.dtype is not x.dtype and t.dtype is not torch.float32:
             raise _lib.StepHipError("layer_norm: %s is %s; %s or float32 wanted" % (name, t.dtype, x.dtype))
-        if t.device != x.device:
+        if t.get_device() != where:
             raise _lib.StepHipError("layer_norm: %s is on %s, x on %s" % (name, t.device, x.device))
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise _lib.StepHipError("layer_norm: weight is %s, bias %s" % (weight.dtype, bias.dtype))
     if not x.is_cuda:
         raise _lib.StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % x.device)
