@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const SmallArgs p) {
 }
 
 // ---------------------------------------------------------------------------------------------- r > 64
-constexpr int TN = 128, KS = 32;                  // columns of an output tile, contraction per stage
+constexpr int KS = 32;                            // contraction per stage
 constexpr int ROWB = 128;                         // bytes of a row's stage: 32 hi, 32 lo
 // scales of X, of A and q(A) A, and of products of one, two and three q(A): elements under 1.21, 1.47, 3.45, 11.9 and 41
 constexpr float SX = 16384.f, SA = 16384.f, SQ[3] = {8192.f, 4096.f, 1024.f};
@@ -431,37 +431,43 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     }
 }
 
-// A wave's 32 MT x 64 share of a tile: the products of the hi parts, and the two small terms in sums of their own, so that the
-// large sum is rounded once per product and not three times.
+// Tiles: 64 MT x 64 NT, a wave's share 32 MT x 32 NT.  MT = 4 and 2 have NT = 2, MT = 1 has 1 (for products too small to fill the CUs).
+template <int MT>
+constexpr int nt_of() {
+    return MT == 1 ? 1 : 2;
+}
+// The products of the hi parts, and the two small terms in sums of their own, so that the large sum is rounded once per product
+// and not three times.
 template <int MT>
 struct Acc {
-    f32x16 v[MT][2], w[MT][2];
+    f32x16 v[MT][nt_of<MT>()], w[MT][nt_of<MT>()];
 };
 template <int MT>
 struct Frag {
-    f16x8 ah[MT], al[MT], bh[2], bl[2];
+    f16x8 ah[MT], al[MT], bh[nt_of<MT>()], bl[nt_of<MT>()];
 };
 template <int MT>
 __device__ __forceinline__ void multiply(Acc<MT>& acc, const Frag<MT>& f) {
+    constexpr int NT = nt_of<MT>();
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[a], f.bh[b], acc.w[a][b], 0, 0, 0);
+        for (int b = 0; b < NT; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[a], f.bh[b], acc.w[a][b], 0, 0, 0);
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc.v[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bh[b], acc.v[a][b], 0, 0, 0);
+        for (int b = 0; b < NT; ++b) acc.v[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bh[b], acc.v[a][b], 0, 0, 0);
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bl[b], acc.w[a][b], 0, 0, 0);
+        for (int b = 0; b < NT; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bl[b], acc.w[a][b], 0, 0, 0);
 }
 
 template <int MT>
 constexpr int stages_of() {
-    return MT == 4 ? 3 : 4;
+    return MT == 4 ? 3 : MT == 2 ? 4 : 6;
 }
-// acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 128) of B over the stages [s0, s1): operands packed alike, K along both.
+// acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 64 NT) of B over the stages [s0, s1): operands packed alike, K along both.
 // A stage lies in LDS as rows of 128 bytes whose eight 16-byte pieces are in the order piece ^ order(row): 16 neighbouring rows
 // are read from different banks (64 banks hold two rows).  Three stages in LDS, copied there directly, two of them in flight.  A wave reads the
 // operands of the next half stage before it multiplies the present one; one barrier a stage, in the middle: before it a
@@ -470,18 +476,19 @@ constexpr int stages_of() {
 // bytes a cycle); 64 x 64 a wave needs 125.
 template <int MT>
 __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
-    constexpr int TM = 64 * MT, STAGE = (TM + TN) * ROWB, NST = stages_of<MT>(), NA = TM / 32, NL = NA + 4;      // copies of a wave: NA + 4 of 8 rows
+    constexpr int NT = nt_of<MT>(), TM = 64 * MT, TN = 64 * NT, STAGE = (TM + TN) * ROWB, NST = stages_of<MT>();
+    constexpr int NA = TM / 32, NB = TN / 32, NL = NA + NB;                  // a wave's copies, of 8 rows each
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, q = lane >> 5;
     const size_t pitch = (size_t)(K / KS) * ROWB;
     const int lrow = lane >> 3, piece = (lane & 7) ^ lrow, order = (l31 & 7) ^ ((l31 >> 3) & 1);
     // a copy's address: the panel's descriptor, this lane's place in it, and a scalar offset
     const __amdgpu_buffer_rsrc_t pa = __builtin_amdgcn_make_buffer_rsrc((void*)(A + (size_t)i0 * pitch), 0, 0xffffffff, 0x00020000);
     const __amdgpu_buffer_rsrc_t pb = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (size_t)j0 * pitch), 0, 0xffffffff, 0x00020000);
-    const unsigned va = (unsigned)((wave * (TM / 4) + lrow) * pitch), vb = (unsigned)((wave * 32 + lrow) * pitch);
+    const unsigned va = (unsigned)((wave * (TM / 4) + lrow) * pitch), vb = (unsigned)((wave * (TN / 4) + lrow) * pitch);
     const unsigned at8[2] = {piece * 16u, (piece ^ 1) * 16u};                // rows 0 .. 7 and 8 .. 15 of each 16
     const unsigned row8 = (unsigned)(8 * pitch);
     char* da = lds + wave * (TM / 4) * ROWB;
-    char* db = lds + TM * ROWB + wave * 32 * ROWB;
+    char* db = lds + TM * ROWB + wave * (TN / 4) * ROWB;
     auto copy = [](__amdgpu_buffer_rsrc_t from, unsigned lane_at, unsigned at, char* to) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, (int)lane_at, (int)at, 0, 0);
     };
@@ -490,10 +497,10 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
 #pragma unroll
         for (int i = 0; i < NA; ++i) copy(pa, va + at8[i & 1], at + i * row8, da + buf * STAGE + i * 1024);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) copy(pb, vb + at8[i & 1], at + i * row8, db + buf * STAGE + i * 1024);
+        for (int i = 0; i < NB; ++i) copy(pb, vb + at8[i & 1], at + i * row8, db + buf * STAGE + i * 1024);
     };
     const char* ra = lds + ((wave >> 1) * (TM / 2) + l31) * ROWB;
-    const char* rb = lds + (TM + (wave & 1) * 64 + l31) * ROWB;
+    const char* rb = lds + (TM + (wave & 1) * (TN / 2) + l31) * ROWB;
     auto read = [&](Frag<MT>& f, int buf, int kk) {
         const int hi = buf * STAGE + (((kk * 2 + q) ^ order) * 16), lo = buf * STAGE + (((4 + kk * 2 + q) ^ order) * 16);
 #pragma unroll
@@ -502,7 +509,7 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
             f.ah[t] = *(const f16x8*)(ra + hi + t * 32 * ROWB);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
             f.bh[t] = *(const f16x8*)(rb + hi + t * 32 * ROWB);
             f.bl[t] = *(const f16x8*)(rb + lo + t * 32 * ROWB);
         }
@@ -520,10 +527,11 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
         __builtin_amdgcn_sched_barrier(0);        // too: else it waits for f1 as well before f0 is used.)
         read(f1, buf, 1);
         multiply(acc, f0);
+        // the reads among the first half of the products: the rest of them covers the last read's way
 #pragma unroll
-        for (int i = 0; i < 2 * MT + 4; ++i) {    // a read, and the matrix cores stay busy behind it
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, MT == 4 ? 2 : 1, 0);
+        for (int i = 0; i < (MT == 4 ? 12 : MT == 2 ? 4 : 1); ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, MT == 4 ? 1 : MT == 2 ? 2 : 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");
@@ -536,8 +544,8 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
         issue(s + NST, buf);
         multiply(acc, f1);
 #pragma unroll
-        for (int i = 0; i < 2 * MT + 4; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+        for (int i = 0; i < (MT == 4 ? 12 : MT == 2 ? 4 : 1); ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, MT == 4 ? 1 : MT == 2 ? 2 : 4, 1);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
         }
 #pragma unroll
@@ -556,11 +564,12 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
 template <int MT, typename F>
 __device__ __forceinline__ void each(const Acc<MT>& acc, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, q = lane >> 5;
-    const int wi = (wave >> 1) * 32 * MT, wj = (wave & 1) * 64;
+    constexpr int NT = nt_of<MT>();
+    const int wi = (wave >> 1) * 32 * MT, wj = (wave & 1) * 32 * NT;
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < NT; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 f(wi + 32 * a + 8 * (e >> 2) + 4 * q + (e & 3), wj + 32 * b + l31, acc.v[a][b][e] + acc.w[a][b][e]);
@@ -569,8 +578,8 @@ __device__ __forceinline__ void each(const Acc<MT>& acc, F f) {
 // The products: what they multiply, and what becomes of `rows` rows of a tile [rows][EP] in LDS that begins at (i0, j0).
 enum Product { XXT, POLY, SYM, UPDATE, RESULT };                             // X X^T; q(s1); s1 s2, commuting; s2 X; s2 X as the result
 
-// tiles of 64 MT x 128 that hold the diagonal of an R x R matrix and what is over it, in blocks of 1024 x 1024 (which share
-// their operands in an XCD's L2): block column after block column
+// tiles that hold the diagonal of an R x R matrix and what is over it, in blocks of 8 tiles' columns squared (which share their
+// operands in an XCD's L2): block column after block column
 __device__ __host__ __forceinline__ int tri_count(int cols, int per) {       // tiles of the first `cols` columns of a block on the diagonal
     int n = 0;
     for (int j = 0; j < cols; ++j) n += j / per + 1;
@@ -578,7 +587,7 @@ __device__ __host__ __forceinline__ int tri_count(int cols, int per) {       // 
 }
 template <int MT>
 __device__ __forceinline__ void tri_tile(int t, int cols, int& ti, int& tj) {
-    constexpr int PER = MT / 2, H = 8 / PER;       // columns of tiles per row of tiles; rows of tiles in a block
+    constexpr int PER = MT / nt_of<MT>(), H = 8 / PER;   // columns of tiles per row of tiles; rows of tiles in a block
     int J = 0;
     for (;; ++J) {
         const int w = cols - 8 * J < 8 ? cols - 8 * J : 8;
@@ -600,8 +609,8 @@ __device__ __forceinline__ void tri_tile(int t, int cols, int& ti, int& tj) {
         t -= n;
     }
 }
-int tri_tiles(int R, int per) {
-    const int cols = R / TN, h = 8 / per;
+int tri_tiles(int cols, int per) {
+    const int h = 8 / per;
     int n = 0;
     for (int J = 0; 8 * J < cols; ++J) {
         const int w = cols - 8 * J < 8 ? cols - 8 * J : 8;
@@ -612,6 +621,7 @@ int tri_tiles(int R, int per) {
 
 template <int PROD, int MT>
 __device__ __forceinline__ void locate(const Big& p, int tile, int& z, int& i0, int& j0, int tiles) {
+    constexpr int TN = 64 * nt_of<MT>();
     z = tile / tiles;
     int t = tile - z * tiles, ti, tj;
     if constexpr (PROD <= SYM) {
@@ -625,17 +635,17 @@ __device__ __forceinline__ void locate(const Big& p, int tile, int& z, int& i0, 
     j0 = tj * TN;
 }
 // pitch of a tile in LDS at the end: rows of 16-byte pieces, or columns in different banks where the result is written by columns
-template <int PROD>
+template <int PROD, int TN>
 constexpr int pitch_of() {
     return PROD == RESULT ? TN + 1 : TN + 4;
 }
 // columns of ROWS rows in LDS as rows of a packed matrix: four neighbouring threads write 64 bytes of a row, and a wave reads at
 // most two values from a bank
-template <int ROWS, int EP, typename F>
+template <int ROWS, int TN, int EP, typename F>
 __device__ __forceinline__ void transposed(const float* sm, F to) {
 #pragma unroll 4
-    for (int u = threadIdx.x; u < ROWS * 16; u += 256) {
-        const int j = ROWS == 8 ? u : (u >> 2) & (TN - 1), i = ROWS == 8 ? 0 : ((u >> 9) * 4 + (u & 3)) * 8;
+    for (int u = threadIdx.x; u < ROWS * TN / 8; u += 256) {
+        const int j = ROWS == 8 ? u : (u >> 2) & (TN - 1), i = ROWS == 8 ? 0 : (u / (4 * TN) * 4 + (u & 3)) * 8;
         char* d = to(i, j);
         if (!d) continue;
         float v[8];
@@ -645,11 +655,11 @@ __device__ __forceinline__ void transposed(const float* sm, F to) {
     }
 }
 
-template <int PROD, int ROWS, typename T>
+template <int PROD, int ROWS, int TN, typename T>
 __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, int j0) {
-    constexpr int N = ROWS == 8 ? 1 : ROWS * 16 / 256, M = N < 8 ? N : 8;     // eight neighbours N times a thread, M of them at a time
-    constexpr int EP = pitch_of<PROD>();
-    const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * 8;
+    constexpr int EP = pitch_of<PROD, TN>(), STEP = 256 / (TN / 8);           // rows that the threads' packs of eight neighbours cover
+    constexpr int N = ROWS < STEP ? 1 : ROWS / STEP, M = N < 8 ? N : 8;      // N times, M of them at a time
+    const int row = threadIdx.x / (TN / 8), col = threadIdx.x % (TN / 8) * 8;
     if constexpr (PROD <= SYM) {
         char* to = p.s3 + (size_t)z * p.RA * p.R * 4;
         const char* a = p.s1 + (size_t)z * p.RA * p.R * 4;
@@ -659,7 +669,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
             if constexpr (PROD == POLY) {
 #pragma unroll
                 for (int k = 0; k < M; ++k) {
-                    const int i = row + 16 * (u + k);
+                    const int i = row + STEP * (u + k);
                     if (i >= ROWS || (i0 + i) / TN > cb) continue;
                     const char* s = packed((char*)a, i0 + i, j0 + col, p.R);
                     hi[k] = *(const f16x8*)s;
@@ -668,7 +678,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
             }
 #pragma unroll
             for (int k = 0; k < M; ++k) {
-                const int i = row + 16 * (u + k);
+                const int i = row + STEP * (u + k);
                 if (i >= ROWS || (i0 + i) / TN > cb) continue;
                 float v[8];
 #pragma unroll
@@ -684,18 +694,18 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
             }
         }
         if constexpr (PROD == POLY) __syncthreads();
-        transposed<ROWS, EP>(sm, [&](int i, int j) { return (i0 + i) / TN >= cb ? nullptr : packed(to, j0 + j, i0 + i, p.R); });
+        transposed<ROWS, TN, EP>(sm, [&](int i, int j) { return (i0 + i) / TN >= cb ? nullptr : packed(to, j0 + j, i0 + i, p.R); });
     } else if constexpr (PROD == UPDATE) {                                   // rows: the long side
         char* xt = p.xt2 + (size_t)z * p.R * p.L * 4;
         char* x = p.x + (size_t)z * p.RA * p.L * 4;
 #pragma unroll 4
-        for (int i = row; i < ROWS; i += 16) {
+        for (int i = row; i < ROWS; i += STEP) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = sm[i * EP + col + e];
             put8(packed(xt, i0 + i, j0 + col, p.R), v);
         }
-        transposed<ROWS, EP>(sm, [&](int i, int j) { return packed(x, j0 + j, i0 + i, p.L); });
+        transposed<ROWS, TN, EP>(sm, [&](int i, int j) { return packed(x, j0 + j, i0 + i, p.L); });
     } else {
         // packs along the matrix's rows: of the tile's columns where the long side is the matrix's rows, of its rows otherwise
         const Io io = shifted(p.io, (size_t)p.m * p.n * z, sizeof(T));
@@ -759,20 +769,21 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
     }
     const int stages = K / KS;
     const int s0 = whole ? 0 : (int)((long long)stages * split / splits), s1 = whole ? stages : (int)((long long)stages * (split + 1) / splits);
+    constexpr int TN = 64 * nt_of<MT>();
     Acc<MT> acc;
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < nt_of<MT>(); ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[a][b][e] = acc.w[a][b][e] = 0.f;
     main_loop(acc, A, B, K, i0, j0, s0, s1, smem);
     const float f = p.scale;
     if (whole) {
         float* sm = (float*)smem;
-        each(acc, [&](int i, int j, float v) { sm[i * pitch_of<PROD>() + j] = v * f; });
+        each(acc, [&](int i, int j, float v) { sm[i * pitch_of<PROD, TN>() + j] = v * f; });
         __syncthreads();
-        finish<PROD, 64 * MT, T>(p, sm, z, i0, j0);
+        finish<PROD, 64 * MT, TN, T>(p, sm, z, i0, j0);
     } else {
         float* slab = p.slab + ((size_t)(tile - full) * splits + split) * (64 * MT * TN);
         each(acc, [&](int i, int j, float v) { slab[i * TN + j] = v * f; });
@@ -781,19 +792,21 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
 // eight rows of a split tile, its shares added in order
 template <int PROD, int MT, typename T>
 __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, int full, int splits) {
-    constexpr int EP = pitch_of<PROD>();
+    constexpr int TN = 64 * nt_of<MT>(), EP = pitch_of<PROD, TN>();
     __shared__ __attribute__((aligned(16))) float sm[8 * EP];
     int z, i0, j0;
     locate<PROD, MT>(p, full + blockIdx.x, z, i0, j0, tiles);
-    const int i = threadIdx.x >> 5, j = (threadIdx.x & 31) * 4;
-    const float* slab = p.slab + (size_t)blockIdx.x * splits * (64 * MT * TN) + (blockIdx.y * 8 + i) * TN + j;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    const int i = threadIdx.x / (TN / 4), j = threadIdx.x % (TN / 4) * 4;
+    if (i < 8) {
+        const float* slab = p.slab + (size_t)blockIdx.x * splits * (64 * MT * TN) + (blockIdx.y * 8 + i) * TN + j;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int s = 0; s < splits; ++s) v += *(const f32x4*)(slab + (size_t)s * 64 * MT * TN);
+        for (int s = 0; s < splits; ++s) v += *(const f32x4*)(slab + (size_t)s * 64 * MT * TN);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sm[i * EP + j + e] = v[e];
+        for (int e = 0; e < 4; ++e) sm[i * EP + j + e] = v[e];
+    }
     __syncthreads();
-    finish<PROD, 8, T>(p, sm, z, i0 + blockIdx.y * 8, j0);
+    finish<PROD, 8, TN, T>(p, sm, z, i0 + blockIdx.y * 8, j0);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -810,8 +823,8 @@ Share share(int mt, long long tiles, long long total) {
     return s;
 }
 double cycles(const Share& s, int stages) {
-    const double one = s.mt == 4 ? 1600 : 850, round = stages * one + 8000;
-    return s.full / CUS * round + (s.rest ? (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + 8000 + 26000 : round) : 0);
+    const double one = s.mt == 4 ? 1600 : s.mt == 2 ? 950 : 420, ends = s.mt == 1 ? 7000 : 12000, round = stages * one + ends;
+    return s.full / CUS * round + (s.rest ? (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + ends + 26000 : round) : 0);
 }
 Share best(const Share& a, const Share& b, int stages) { return cycles(b, stages) < cycles(a, stages) ? b : a; }
 Share fastest(int mt, long long tiles, int nb, int stages) {
@@ -831,13 +844,22 @@ struct Layout {
 };
 Layout layout_of(int nb, int r, int l) {
     Layout o{};
-    o.R = step::round_up(r, TN);
+    o.R = step::round_up(r, 128);
     o.L = step::round_up(l, 256);
     o.RA = step::round_up(r, 256);
-    const int t4 = tri_tiles(o.R, 2), t2 = tri_tiles(o.R, 1), sx = o.L / KS, sr = o.R / KS;
-    o.xxt = best(fastest(4, t4, nb, sx), fastest(2, t2, nb, sx), sx);
-    o.sym = best(fastest(4, t4, nb, sr), fastest(2, t2, nb, sr), sr);
-    o.update = best(fastest(4, (long long)(o.L / 256) * (o.R / TN), nb, sr), fastest(2, (long long)(o.L / 128) * (o.R / TN), nb, sr), sr);
+    const int sx = o.L / KS, sr = o.R / KS;
+    auto of = [&](bool tri, int stages) {
+        Share s{};
+        for (int mt : {4, 2, 1}) {
+            const int nt = mt == 1 ? 1 : 2, cols = o.R / (64 * nt);
+            const Share t = fastest(mt, tri ? tri_tiles(cols, mt / nt) : (long long)(o.L / (64 * mt)) * cols, nb, stages);
+            s = mt == 4 ? t : best(s, t, stages);
+        }
+        return s;
+    };
+    o.xxt = of(true, sx);
+    o.sym = of(true, sr);
+    o.update = of(false, sr);
     return o;
 }
 // workspace of a stack of `batch` matrices with r > 64, `sub` of them at a time
@@ -869,7 +891,7 @@ Layout layout(int batch, int m, int n) {
     for (int i = 0; i < (o.group > 1 ? 4 : 2); ++i) o.r[i] = take(sub * RA * R * 4);
     // shares of split tiles: fewer than one a CU, of 256 x 128 at most.  A last part of the batch that is smaller is shared out anew.
     const bool any = sub < batch || o.xxt.splits > 1 || o.sym.splits > 1 || o.update.splits > 1;
-    o.slab = take(any ? (size_t)CUS * 256 * TN * 4 : 0);
+    o.slab = take(any ? (size_t)CUS * 256 * 128 * 4 : 0);
     o.total = at;
     return o;
 }
@@ -945,7 +967,7 @@ int check(const step_ns_item* items, int count) {
 template <int PROD, int MT, typename T>
 int product_of(const Big& p, const Share& s, hipStream_t st) {
     auto kern = ns_product_kernel<PROD, MT, T>;
-    constexpr size_t lds = stages_of<MT>() * (64 * MT + TN) * ROWB;
+    constexpr size_t lds = stages_of<MT>() * 64 * (MT + nt_of<MT>()) * ROWB;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
@@ -957,7 +979,7 @@ int product_of(const Big& p, const Share& s, hipStream_t st) {
 }
 template <int PROD, typename T>
 int product(const Big& p, const Share& s, hipStream_t st) {
-    return s.mt == 4 ? product_of<PROD, 4, T>(p, s, st) : product_of<PROD, 2, T>(p, s, st);
+    return s.mt == 4 ? product_of<PROD, 4, T>(p, s, st) : s.mt == 2 ? product_of<PROD, 2, T>(p, s, st) : product_of<PROD, 1, T>(p, s, st);
 }
 template <typename T>
 int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
