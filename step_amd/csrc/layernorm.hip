@@ -399,7 +399,7 @@ extern "C" size_t step_layernorm_bwd_ws_bytes(long long rows, int cols) {
 extern "C" int step_layernorm_fwd(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd,
                                   long long rows, int cols, int dtype, int wdtype, float eps, void* stream) {
     STEP_REQUIRE(x && y, "step_layernorm_fwd: null pointer");
-    STEP_REQUIRE(rows >= 1 && cols >= 1, "step_layernorm_fwd: bad shape rows=%lld cols=%d", rows, cols);
+    STEP_REQUIRE(rows >= 1 && cols >= 1 && cols <= 1 << 28, "step_layernorm_fwd: bad shape rows=%lld cols=%d", rows, cols);
     STEP_REQUIRE(elem_bytes(dtype) && elem_bytes(wdtype), "step_layernorm_fwd: unknown type %d / %d", dtype, wdtype);
     STEP_REQUIRE(wdtype == STEP_F32 || wdtype == dtype, "step_layernorm_fwd: weights of type %d beside rows of type %d", wdtype, dtype);
     STEP_REQUIRE((mean == nullptr) == (rstd == nullptr), "step_layernorm_fwd: mean and rstd come together");
@@ -432,7 +432,7 @@ extern "C" int step_layernorm_bwd(const void* dy, const void* x, const void* w, 
                                   void* dx, void* dw, void* db, long long rows, int cols, int dtype, int wdtype, void* ws,
                                   size_t ws_bytes, void* stream) {
     STEP_REQUIRE(dy && x && mean && rstd, "step_layernorm_bwd: null pointer");
-    STEP_REQUIRE(rows >= 1 && cols >= 1, "step_layernorm_bwd: bad shape rows=%lld cols=%d", rows, cols);
+    STEP_REQUIRE(rows >= 1 && cols >= 1 && cols <= 1 << 28, "step_layernorm_bwd: bad shape rows=%lld cols=%d", rows, cols);
     STEP_REQUIRE(elem_bytes(dtype) && elem_bytes(wdtype), "step_layernorm_bwd: unknown type %d / %d", dtype, wdtype);
     STEP_REQUIRE(wdtype == STEP_F32 || wdtype == dtype, "step_layernorm_bwd: weights of type %d beside rows of type %d", wdtype, dtype);
     const bool sums = dw || db;

@@ -744,11 +744,14 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
 template <int PROD, int MT, typename T>
 __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int tiles, int full, int splits) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int tile = blockIdx.x, split = 0;
-    if (tile < full) tile = (tile & 7) * (full >> 3) + (tile >> 3);          // an XCD's tiles are neighbours
+    // blocks go to the eight XCDs in turn: each gets neighbouring tiles, whose operands its L2 then holds
+    auto neighbours = [](int b, int n) { return (b & 7) * (n >> 3) + min(b & 7, n & 7) + (b >> 3); };
+    int tile, split = 0;
+    if ((int)blockIdx.x < full) tile = neighbours(blockIdx.x, full);
     else {
-        split = (tile - full) % splits;
-        tile = full + (tile - full) / splits;
+        const int rest = ((int)gridDim.x - full) / splits, u = neighbours((int)blockIdx.x - full, (int)gridDim.x - full);
+        split = u / rest;
+        tile = full + u % rest;
     }
     const bool whole = (int)blockIdx.x < full || splits == 1;
     int z, i0, j0;
@@ -767,7 +770,7 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
         B = p.s2 + (size_t)z * p.RA * p.R * 4;
         K = p.R;
     }
-    const int stages = K / KS;
+    const int stages = ((PROD == XXT ? p.l : p.r) + KS - 1) / KS;            // (behind them is nothing but zeros)
     const int s0 = whole ? 0 : (int)((long long)stages * split / splits), s1 = whole ? stages : (int)((long long)stages * (split + 1) / splits);
     constexpr int TN = 64 * nt_of<MT>();
     Acc<MT> acc;
@@ -847,7 +850,7 @@ Layout layout_of(int nb, int r, int l) {
     o.R = step::round_up(r, 128);
     o.L = step::round_up(l, 256);
     o.RA = step::round_up(r, 256);
-    const int sx = o.L / KS, sr = o.R / KS;
+    const int sx = step::ceil_div(l, KS), sr = step::ceil_div(r, KS);
     auto of = [&](bool tri, int stages) {
         Share s{};
         for (int mt : {4, 2, 1}) {

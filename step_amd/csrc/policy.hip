@@ -399,7 +399,7 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
                                 float* loss, float* stats, float* logp, void* dlogits, long long rows, int classes,
                                 int dtype, void* ws, size_t ws_bytes, void* stream) {
     STEP_REQUIRE(logits && actions && old_logp && advantages && ws, "step_policy_loss: null pointer");
-    STEP_REQUIRE(rows >= 1 && classes >= 1 && classes <= 0x7fffff00, "step_policy_loss: bad shape rows=%lld classes=%d", rows, classes);
+    STEP_REQUIRE(rows >= 1 && classes >= 1 && classes <= 1 << 30, "step_policy_loss: bad shape rows=%lld classes=%d", rows, classes);
     STEP_REQUIRE(elem_bytes(dtype), "step_policy_loss: unknown type %d", dtype);
     STEP_REQUIRE(upstream ? dlogits != nullptr : loss && stats && logp, "step_policy_loss: null output");
     STEP_REQUIRE((((uintptr_t)logits | (uintptr_t)dlogits) & (elem_bytes(dtype) - 1)) == 0, "step_policy_loss: logits or dlogits lie across elements");
