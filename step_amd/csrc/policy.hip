@@ -39,17 +39,17 @@ struct Args {
     double clip_low, clip_high, beta;   // a clipped ratio's 1.2 in fp32 is off by 4e-8, the same way in every row
 };
 
-// maximum and sum of exponentials about it, joined over the G threads of a row, in base 2: m is the row's largest logit
-// times log2 e, rounded once and from there on exact, an element's exponent x log2 e - m is one fused operation
+// maximum and sum of exponentials about it, joined over the G threads of a row.  The maximum is taken off before the multiplication
+// by log2 e: the type's lowest values, as masks write them, times log2 e would overflow.
 struct Soft {
     float m, s;
 };
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float exp_of(float x, float m) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, L2E, -m)); }
+__device__ __forceinline__ float exp_of(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * L2E); }
 // for the sum, whose logarithm the loss hangs on: with the rest of log2 e too (fp32's log2 e alone is off by 1.3e-8, the same
 // way for all elements)
 __device__ __forceinline__ float exp_for_sum(float x, float m) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(x, L2E_REST, __builtin_fmaf(x, L2E, -m)));
+    const float d = x - m;
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, L2E_REST, d * L2E));
 }
 __device__ __forceinline__ float finite_or_0(float m) { return m == -__builtin_inff() ? 0.f : m; }   // no -inf - -inf
 
@@ -66,7 +66,7 @@ __device__ __forceinline__ Soft join(const Soft w, Soft* sm) {
         const float m0 = finite_or_0(r.m);
         r.s = 0.f;
 #pragma unroll
-        for (int i = 0; i < G / 64; ++i) r.s += sm[i].s * exp_of(sm[i].m - m0);
+        for (int i = 0; i < G / 64; ++i) r.s += sm[i].s * exp_of(sm[i].m, m0);
         return r;
     }
 }
@@ -113,7 +113,7 @@ __device__ __forceinline__ double exp_of64(double x) {
 // the row's scalars: returns dL/dlp / count (times the upstream gradient), adds the row to the block's sums
 __device__ __forceinline__ float row_scalars(const Args& p, long long row, Soft f, float za, bool valid, double count,
                                              double* sums) {
-    const double lp = valid ? (double)za - ((double)f.m + log2_of(f.s)) * LN2 : (double)__builtin_nanf("");
+    const double lp = valid ? (double)za - (double)f.m - log2_of(f.s) * LN2 : (double)__builtin_nanf("");
     const double a = p.adv[row], ratio = exp_of64(lp - (double)p.old_logp[row]);
     const double lo = 1.0 - p.clip_low, hi = 1.0 + p.clip_high;
     const double o1 = ratio * a, o2 = (ratio > hi ? hi : ratio < lo ? lo : ratio) * a;   // a NaN stays one
@@ -148,9 +148,9 @@ __device__ __forceinline__ void add_to(Soft& f, const Pack<T, N>* q, int packs) 
     for (int k = 0; k < packs; ++k)
 #pragma unroll
         for (int e = 0; e < N; ++e) m = fmaxf(m, (float)q[k].v[e]);
-    m = fmaxf(f.m, m * L2E);
+    m = fmaxf(f.m, m);
     const float m0 = finite_or_0(m);
-    float s0 = f.s * exp_of(f.m - m0), s1 = 0.f;             // two chains
+    float s0 = f.s * exp_of(f.m, m0), s1 = 0.f;             // two chains
 #pragma unroll
     for (int k = 0; k < packs; ++k)
 #pragma unroll
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
             }
         }
         const float m = wave_reduce<G>(f.m, larger);
-        f.s = wave_reduce<G>(f.s * exp_of(f.m - finite_or_0(m)), sum);
+        f.s = wave_reduce<G>(f.s * exp_of(f.m, finite_or_0(m)), sum);
         f.m = m;
         f = join<G>(f, sm[turn]);
         turn ^= 1;
@@ -280,19 +280,12 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
         } else {
             constexpr int U = 8;
             for (int c0 = 0; c0 < p.classes; c0 += U * G * N) {
+                const Columns<N, U, G, U> part{p.classes - c0, lane};   // (each of the last packs may lie before c0)
                 Pack<T, N> q[U];
+                part.load(q, z + c0);
 #pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const int c = c0 + (k * G + lane) * N;
-                    q[k] = load_pack<T, N>(z + (c < p.classes - N ? c : p.classes - N));
-                }
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const int c = c0 + (k * G + lane) * N;
-                    if (c < p.classes) store_pack<T, N>(g + (c < p.classes - N ? c : p.classes - N), gradient_of<T, N>(q[k], f.m, scale));
-                }
+                for (int k = 0; k < U; ++k) part.store(g + c0, k, gradient_of<T, N>(q[k], f.m, scale));
             }
-            __syncthreads();                                 // (packs overlap at the row's end)
         }
         // the thread that wrote the action's element writes it once more
         if (valid && lane == action / N % G) g[action] = (T)(exp_of((float)z[action], f.m) * scale + coef);

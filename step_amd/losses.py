@@ -67,7 +67,7 @@ def vae_loss(x_in, x_out, mean, lsig, beta=1.):
 class _PolicyLossFn(torch.autograd.Function):
     """The forward leaves the gradient for an upstream gradient of 1 behind (value and gradient take one pass over the
     logits); the backward hands it out, or computes it again from the logits where the upstream gradient is not 1 - on
-    the device, with one rounding - or where a retained graph asks a second time."""
+    the device, with one rounding - or where a retained graph asks a second time, or a captured backward without its forward."""
 
     @staticmethod
     def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, beta):
@@ -90,7 +90,7 @@ class _PolicyLossFn(torch.autograd.Function):
                       loss, stats, logp, grad, rows, classes, _lib.DTYPES[z.dtype], ws, nb)
         if need:
             ctx.save_for_backward(z, actions, old_logp, advantages, ref_logp, mask)
-            ctx.grad, ctx.ws = grad, ws
+            ctx.grad, ctx.ws, ctx.captured = grad, ws, z.is_cuda and torch.cuda.is_current_stream_capturing()
         return loss, logp, stats
 
     @staticmethod
@@ -98,7 +98,8 @@ class _PolicyLossFn(torch.autograd.Function):
     def backward(ctx, g, _logp, _stats):
         z, actions, old_logp, advantages, ref_logp, mask = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
-        first = grad is not None
+        # a graph of the backward alone keeps no hold on the forward's memory, and is replayed without it
+        first = grad is not None and (ctx.captured or not torch.cuda.is_current_stream_capturing())
         if not first:
             grad = torch.empty_like(z)
         rows = z.numel() // z.shape[-1]
@@ -126,6 +127,8 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
         raise _lib.StepHipError("policy_loss: logits (..., classes) wanted")
     if logits.dtype not in _lib.DTYPES:
         raise _lib.StepHipError("policy_loss: float32, bfloat16 or float16 logits wanted, got %s" % logits.dtype)
+    if logits.shape[-1] > 1 << 30:
+        raise _lib.StepHipError("policy_loss: %d classes, 2^30 at most" % logits.shape[-1])
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     low, high, beta = float(low), float(high), float(beta)
     if not (0.0 <= low <= 1.0 and high >= 0.0):

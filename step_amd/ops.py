@@ -854,6 +854,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     shape = x.shape
     if not shape or shape[-1] < 1:
         raise _lib.StepHipError("layer_norm: x %s has no last axis to normalise" % (tuple(shape),))
+    if shape[-1] > 1 << 28:
+        raise _lib.StepHipError("layer_norm: %d columns, 2^28 at most" % shape[-1])
     if x.dtype not in _lib.DTYPES:
         raise _lib.StepHipError("layer_norm: float32, bfloat16 or float16 wanted, got %s" % x.dtype)
     where = x.get_device()

@@ -51,6 +51,8 @@ def newton_schulz(g, steps=STEPS, eps=EPS):
         if t.dtype != gs[0].dtype or t.device != gs[0].device:
             raise _lib.StepHipError("newton_schulz: a list has one type and one device, got %s on %s and %s on %s" % (
                 gs[0].dtype, gs[0].device, t.dtype, t.device))
+        if t.numel() > 0 and (max(t.shape[-2:]) > 1 << 21 or t.numel() // (t.shape[-2] * t.shape[-1]) > 1 << 24):
+            raise _lib.StepHipError("newton_schulz: %s: 2^21 rows or columns and 2^24 matrices at most" % (tuple(t.shape),))
     for t in gs:
         if not t.is_cuda:
             raise _lib.StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % t.device)
@@ -78,7 +80,8 @@ class Muon(torch.optim.Optimizer):
     Parameters of one axis (biases, norms' weights) and those of a group with ``matrices=False`` take Adam steps with decoupled
     decay at ``adam_lr`` (default: lr), ``adam_betas``, ``adam_eps``.  All parameters are fp32, contiguous and on one GPU per
     step; those without a gradient are left alone.  The matrices' step is one library call, three launches for all matrices
-    with a side of at most 64."""
+    with a side of at most 64.  It may be captured into a graph once every matrix has had a step (lr and the other options are
+    then those of the capture); Adam's part may not."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=STEPS, eps=EPS, adam_lr=None,
                  adam_betas=(0.9, 0.999), adam_eps=1e-8):
@@ -122,17 +125,23 @@ class Muon(torch.optim.Optimizer):
                 raise _lib.StepHipError("Muon: the parameters of a group lie on %s and %s" % (dev, p.device))
             if not p.is_contiguous():
                 raise _lib.StepHipError("Muon: non-contiguous parameter of shape %s" % (tuple(p.shape),))
+        if len({p.data_ptr() for p in mats}) != len(mats):       # two updates of one matrix at a time
+            raise _lib.StepHipError("Muon: a group holds a parameter twice")
         items, keep, written = [], [], []
         for p in mats:
             state = self.state[p]
             buf = state.get("momentum_buffer")
             if buf is None:
+                if torch.cuda.is_current_stream_capturing():     # (a replay would clear it again)
+                    raise _lib.StepHipError("Muon: take one step before a capture, which makes the momentum buffers")
                 buf = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             elif buf.dtype is not torch.float32 or buf.shape != p.shape or buf.device != dev or not buf.is_contiguous():
                 raise _lib.StepHipError("Muon: momentum buffer %s %s does not fit its parameter" % (buf.dtype, tuple(buf.shape)))
             g = p.grad.contiguous()
             m = p.shape[0]
             n = p.numel() // m
+            if max(m, n) > 1 << 21:
+                raise _lib.StepHipError("Muon: a parameter of shape %s: 2^21 rows or columns at most" % (tuple(p.shape),))
             keep.append(g)
             written += (p, buf)
             items.append((g.data_ptr(), None, buf.data_ptr(), p.data_ptr(), 1, m, n, math.sqrt(m / n) if m > n else 1.0))
@@ -143,6 +152,8 @@ class Muon(torch.optim.Optimizer):
     def _step_rest(self, group, rest):
         lr = group["lr"] if group["adam_lr"] is None else group["adam_lr"]
         b1, b2 = group["adam_betas"]
+        if rest[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            raise _lib.StepHipError("Muon: Adam's corrections are counted on the host: only the matrices' step can be captured")
         grads, firsts, seconds = [p.grad for p in rest], [], []
         for p in rest:
             state = self.state[p]

@@ -165,3 +165,20 @@ def test_harness_and_head_arguments():
     plain, layer = (Classifier(3, 29, 4, {"strategy": "spatial"}, **kw).state_dict() for kw in ({}, {"head_norm": "layer"}))
     assert set(plain) - set(layer) == {"data_bn2.running_mean", "data_bn2.running_var", "data_bn2.num_batches_tracked"}
     assert not set(layer) - set(plain)
+
+
+def test_sizes_beyond_the_library_are_refused():
+    """whose counts are C ints: nothing is cut off silently"""
+    huge = lambda *s: torch.empty(s, dtype=torch.bfloat16, device="meta")  # noqa: E731
+    with pytest.raises(StepHipError, match="columns"):
+        ops.layer_norm(huge(1, (1 << 32) + 5))
+    with pytest.raises(StepHipError, match="classes"):
+        losses.policy_loss(huge(1, (1 << 32) + 5), huge(1), huge(1), huge(1))
+    for shape in ((1, (1 << 32) + 5), ((1 << 32) + 5, 3), ((1 << 32) + 1, 2, 2)):
+        with pytest.raises(StepHipError, match="at most"):
+            optim.newton_schulz(huge(*shape))
+    for name, at in (("step_layernorm_fwd", 7), ("step_policy_loss", 16)):
+        args = {"step_layernorm_fwd": [PTR, None, None, PTR, None, None, 4, 8, 0, 0, 1e-5, None],
+                "step_policy_loss": [PTR, PTR, PTR, PTR, None, None, 0.2, 0.2, 0.0, None, 0, PTR, PTR, PTR, PTR, 4, 8, 0, PTR, 1 << 20, None]}[name]
+        args[at] = (1 << 31) - 1
+        assert code(name, *args)[0] == -1

@@ -290,3 +290,55 @@ def test_inference_caches_see_a_step():
         fresh.load_state_dict(m.state_dict())
         want, _ = fresh(x)
     assert torch.equal(after, want) and not torch.equal(after, before)
+
+
+# The products' tiles are 64 x 64, 128 x 128 or 256 x 128, whole, split along the contraction, or both; l >= 2 r takes up to
+# three steps together.  Tolerance: the above with the contraction K = max(m, n), whose sums' roundings grow with its root.
+@pytest.mark.parametrize("shape,dtype", [
+    ((513, 3590), torch.float32), ((3590, 513), torch.bfloat16),     # 128 x 128 split 17 times
+    ((2970, 2409), torch.float32),                                   # 128 x 128
+    ((1781, 2810), torch.float32), ((1781, 2810), torch.float16),    # 256 x 128 split 4 times
+    ((3048, 3035), torch.float32), ((3048, 3035), torch.bfloat16),   # whole rounds and split tiles of each kind
+    ((449, 1941), torch.float16), ((150, 9001), torch.float32), ((9001, 130), torch.float32),
+    ((9, 269, 2656), torch.bfloat16), ((8, 1157, 416), torch.float32), ((3, 1801, 600), torch.float32)])
+def test_larger(shape, dtype):
+    from step_amd import optim
+    m, n = shape[-2:]
+    g = matrices(*shape, seed=m, dtype=dtype)
+    tol = torch.finfo(dtype).eps / 2 + 2.5e-5 * max(1.0, math.sqrt(max(m, n) / 600))
+    close(optim.newton_schulz(g), orthogonalised(g), tol, shape)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 8])
+def test_steps_taken_together(steps):
+    """three steps together cost the smallest singular values up to 2e-5 more; a step more may multiply by 1.7"""
+    from step_amd import optim
+    for m, n in ((70, 300), (901, 110)):
+        g = matrices(m, n)
+        close(optim.newton_schulz(g, steps=steps), orthogonalised(g, steps), tolerance(m, n, torch.float32) * (2 if steps < 6 else 5), (m, n))
+
+
+def test_muon_refuses_what_it_cannot_do():
+    from step_amd import optim
+    p = torch.nn.Parameter(matrices(20, 30))
+    alias = torch.nn.Parameter(p.detach())                    # the same memory
+    for q in (p, alias):
+        q.grad = matrices(20, 30, seed=1)
+    before = p.detach().clone()
+    with pytest.raises(optim._lib.StepHipError, match="twice"):
+        optim.Muon([p, alias]).step()
+    assert torch.equal(p, before)
+    fresh, bias = optim.Muon([p]), optim.Muon([p, torch.nn.Parameter(torch.zeros(3, device=D))])
+    bias.param_groups[0]["params"][1].grad = torch.ones(3, device=D)
+    bias.step()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for opt, what in ((fresh, "one step before"), (bias, "counted on the host")):
+        # (inside the capture, so that it ends in order)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(optim._lib.StepHipError, match=what):
+                opt.step()
+            p.detach().add_(0.0)
+    torch.cuda.synchronize()
+    assert not fresh.state.get(p)

@@ -255,3 +255,38 @@ def test_offsets_beyond_32_bits():
     small, slp, _, sgrad = check(tail, a4, old4, adv4, None, None, beta=0.0)
     assert torch.equal(loss, small) and torch.equal(logp[-4:], slp) and torch.equal(grad[-4:], sgrad)
     assert not grad[-6:-4].any() and not grad[0].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [4, 100, 4000, 70003, 140001])
+def test_the_lowest_values_as_masks(classes, dtype):
+    """classes shut out with the type's lowest value, which times log2 e is beyond fp32; a row that shuts out all of them is
+    uniform, by the definition"""
+    z, a, old, adv, ref, _ = inputs((5,), classes, dtype, seed=classes)
+    lowest = torch.finfo(dtype).min
+    z[1, 1:] = lowest
+    a[1] = 0
+    z[2] = lowest
+    z[3, : classes // 2] = lowest
+    z[4, -1] = torch.finfo(dtype).max
+    a[3:] = classes - 1
+    lp = torch.log_softmax(z.double(), 1).gather(1, a[:, None])[:, 0]
+    check(z, a, (lp + 0.1).float(), adv, (lp - 0.1).float(), None)
+
+
+def test_a_captured_backward_without_its_forward(monkeypatch):
+    """the forward ran eagerly, its gradient's memory is not the graph's: a backward under capture takes memory of its own and
+    computes the gradient anew"""
+    from step_amd import losses
+    z, a, old, adv, ref, mask = inputs((60,), 333, torch.bfloat16)
+    leaf = z.clone().requires_grad_(True)
+    loss = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+    held = loss.grad_fn.grad.data_ptr()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    (captured,) = torch.autograd.grad(loss, leaf, retain_graph=True)
+    assert captured.data_ptr() != held
+    monkeypatch.undo()
+    again = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+    held = again.grad_fn.grad.data_ptr()
+    (want,) = torch.autograd.grad(again, leaf)
+    assert want.data_ptr() == held and torch.equal(captured, want)
