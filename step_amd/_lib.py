@@ -111,7 +111,7 @@ SIGNATURES = {
     "step_layernorm_fwd": (I, [P, P, P, P, P, P, LL, I, I, I, F, P]),
     "step_layernorm_bwd_ws_bytes": (Z, [LL, I]),
     "step_layernorm_bwd": (I, [P, P, P, P, P, P, P, P, LL, I, I, I, P, Z, P]),
-    "step_policy_loss_ws_bytes": (Z, [LL]),
+    "step_policy_loss_ws_bytes": (Z, [LL, I]),
     "step_policy_loss": (I, [P, P, P, P, P, P, DBL, DBL, DBL, P, I, P, P, P, P, LL, I, I, P, Z, P]),
     "step_newton_schulz_ws_bytes": (Z, [P, I]),
     "step_newton_schulz": (I, [P, I, I, I, F, F, I, F, F, P, Z, P]),

@@ -112,7 +112,7 @@ __device__ __forceinline__ double exp_of64(double x) {
 
 // the row's scalars: returns dL/dlp / count (times the upstream gradient), adds the row to the block's sums
 __device__ __forceinline__ float row_scalars(const Args& p, long long row, Soft f, float za, bool valid, double count,
-                                             double* sums) {
+                                             double* sums, bool write = true) {
     const double lp = valid ? (double)za - (double)f.m - log2_of(f.s) * LN2 : (double)__builtin_nanf("");
     const double a = p.adv[row], ratio = exp_of64(lp - (double)p.old_logp[row]);
     const double lo = 1.0 - p.clip_low, hi = 1.0 + p.clip_high;
@@ -127,8 +127,8 @@ __device__ __forceinline__ float row_scalars(const Args& p, long long row, Soft 
     sums[0] += clipped ? -o2 : -o1;
     sums[1] += kl;
     sums[2] += clipped ? 1.0 : 0.0;
-    if (!p.upstream) p.logp[row] = (float)lp;
-    else slope *= (double)*p.upstream;
+    if (p.upstream) slope *= (double)*p.upstream;
+    else if (write) p.logp[row] = (float)lp;
     return (float)(slope / count);
 }
 
@@ -191,15 +191,34 @@ __device__ __forceinline__ void forget(Pack<T, N>& v) {
     }
 }
 
-// G threads a row, NV packs of N elements a thread (the last LAST of them may not fit); NV = 0: the row is read twice
+template <typename T, int N, int NV>
+__device__ __forceinline__ void add_packs(Soft& f, Pack<T, N>* v) {
+    constexpr int U = N == 4 && NV % 2 == 0 ? 2 : 1;         // eight elements at a time
+#pragma unroll
+    for (int i = 0; i < NV; i += U) {
+        add_to<T, N>(f, v + i, U);
+#pragma unroll
+        for (int k = 0; k < U; ++k) forget(v[i + k]);
+    }
+}
+// over the G threads that have the maximum and sum of their elements, the same bits in all of them
+template <int G>
+__device__ __forceinline__ Soft reduce(Soft f, Soft* sm) {
+    const float m = wave_reduce<G < 64 ? G : 64>(f.m, [](float a, float b) { return fmaxf(a, b); });
+    f.s = wave_reduce<G < 64 ? G : 64>(f.s * exp_of(f.m, finite_or_0(m)), [](float a, float b) { return a + b; });
+    f.m = m;
+    return join<G>(f, sm);
+}
+
+// G threads a row, NV packs of N elements a thread (the last LAST of them may not fit)
 template <typename T, int N, int NV, int LAST, int G>
 __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_kernel(const Args p) {
-    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G, KEEP = NV ? NV : 1;
+    constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
     __shared__ Soft sm[2][G > 64 ? G / 64 : 1];
     __shared__ float coef_s;
     if (p.upstream && p.skip_one && *p.upstream == 1.f) return;
     const int lane = threadIdx.x % G;
-    const Columns<N, KEEP, G, LAST> own{p.classes, lane};
+    const Columns<N, NV, G, LAST> own{p.classes, lane};
     const double live_rows = p.count ? *p.count : (double)p.rows, count = live_rows > 1.0 ? live_rows : 1.0;
     double sums[3] = {0.0, 0.0, 0.0};
     int turn = 0;
@@ -221,45 +240,13 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
         const long long a64 = p.actions[row];
         const bool valid = a64 >= 0 && a64 < p.classes;
         const int action = valid ? (int)a64 : -1;
-        Pack<T, N> v[KEEP];
+        Pack<T, N> v[NV];
         Soft f{-__builtin_inff(), 0.f};
-        if constexpr (NV > 0) own.load(v, z);
+        own.load(v, z);
         const float za = lane == 0 && valid ? (float)z[action] : 0.f;
-        auto larger = [](float a, float b) { return fmaxf(a, b); };
-        auto sum = [](float a, float b) { return a + b; };
-        if constexpr (NV > 0) {
-            own.fill(v, (T)-__builtin_inff());
-            constexpr int U = N == 4 && NV % 2 == 0 ? 2 : 1; // eight elements at a time
-#pragma unroll
-            for (int i = 0; i < NV; i += U) {
-                add_to<T, N>(f, v + i, U);
-#pragma unroll
-                for (int k = 0; k < U; ++k) forget(v[i + k]);
-            }
-        } else {
-            constexpr int U = 8;                             // packs in flight
-            for (int c0 = 0; c0 < p.classes; c0 += U * G * N) {
-                Pack<T, N> q[U];
-                int at[U];
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const int c = c0 + (k * G + lane) * N;
-                    at[k] = c < p.classes - N ? c : p.classes - N;
-                    q[k] = load_pack<T, N>(z + at[k]);
-                }
-                if (c0 + U * G * N > p.classes)
-#pragma unroll
-                    for (int k = 0; k < U; ++k)
-#pragma unroll
-                        for (int e = 0; e < N; ++e) q[k].v[e] = at[k] + e >= c0 + (k * G + lane) * N ? q[k].v[e] : (T)-__builtin_inff();
-#pragma unroll
-                for (int k = 0; k < U; ++k) add_to<T, N>(f, q + k, 1);
-            }
-        }
-        const float m = wave_reduce<G>(f.m, larger);
-        f.s = wave_reduce<G>(f.s * exp_of(f.m, finite_or_0(m)), sum);
-        f.m = m;
-        f = join<G>(f, sm[turn]);
+        own.fill(v, (T)-__builtin_inff());
+        add_packs<T, N, NV>(f, v);
+        f = reduce<G>(f, sm[turn]);
         turn ^= 1;
         float coef;
         if constexpr (G <= 64) {
@@ -274,23 +261,85 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
         }
         if (!g) continue;
         const float scale = -coef / f.s;
-        if constexpr (NV > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) own.store(g, i, gradient_of<T, N>(v[i], f.m, scale));
-        } else {
-            constexpr int U = 8;
-            for (int c0 = 0; c0 < p.classes; c0 += U * G * N) {
-                const Columns<N, U, G, U> part{p.classes - c0, lane};   // (each of the last packs may lie before c0)
-                Pack<T, N> q[U];
-                part.load(q, z + c0);
-#pragma unroll
-                for (int k = 0; k < U; ++k) part.store(g + c0, k, gradient_of<T, N>(q[k], f.m, scale));
-            }
-        }
+        for (int i = 0; i < NV; ++i) own.store(g, i, gradient_of<T, N>(v[i], f.m, scale));
         // the thread that wrote the action's element writes it once more
         if (valid && lane == action / N % G) g[action] = (T)(exp_of((float)z[action], f.m) * scale + coef);
     }
     if (!p.upstream) block_sums<BLOCK>(p.part, sums);
+}
+
+// Rows too long for the registers of 1024 threads, in parts of at most PART_PACKS packs a thread: first each part's maximum and
+// sum, then, from the row's parts together, its scalars and the part's gradient - the row is read twice.  The parts fill the
+// card where there are few rows (640 x 140001 bf16: 120 us, 145 with a block of 1024 threads a row;
+// 2000 x 100000 fp32: 465 us, 5.2 TB/s of what it reads and writes; 4 or 16 packs: within 4 % either way).
+constexpr int PART_PACKS = 8;
+template <typename T, int N, bool GRAD>
+__global__ __launch_bounds__(256) void policy_parts_kernel(const Args p, Soft* soft, int parts, int span) {
+    __shared__ Soft sm[2][4];
+    __shared__ float coef_s[2];
+    if (p.upstream && p.skip_one && *p.upstream == 1.f) return;
+    const int tid = threadIdx.x;
+    const double live_rows = p.count ? *p.count : (double)p.rows, count = live_rows > 1.0 ? live_rows : 1.0;
+    double sums[3] = {0.0, 0.0, 0.0};
+    int turn = 0;
+    for (long long item = blockIdx.x; item < p.rows * parts; item += gridDim.x) {
+        const long long row = item / parts;
+        const int part = (int)(item - row * parts), c0 = part * span;
+        const Columns<N, PART_PACKS, 256, PART_PACKS> own{span < p.classes - c0 ? span : p.classes - c0, tid};
+        const T* z = (const T*)p.logits + (size_t)row * p.classes;
+        T* g = GRAD && p.dlogits ? (T*)p.dlogits + (size_t)row * p.classes : nullptr;
+        if (GRAD && !g && part) continue;                    // only the row's scalars are asked for
+        if (p.mask && !p.mask[row]) {
+            if (GRAD && part == 0 && tid == 0 && !p.upstream) p.logp[row] = 0.f;
+            if (g) {
+                Pack<T, N> zero;
+#pragma unroll
+                for (int e = 0; e < N; ++e) zero.v[e] = (T)0.f;
+#pragma unroll
+                for (int i = 0; i < PART_PACKS; ++i) own.store(g + c0, i, zero);
+            }
+            continue;
+        }
+        Pack<T, N> v[PART_PACKS];
+        if (!GRAD || g) own.load(v, z + c0);                 // (a pack at the end of a short last part lies in the part before)
+        Soft f{-__builtin_inff(), 0.f};
+        if constexpr (!GRAD) {
+            own.fill(v, (T)-__builtin_inff());
+            add_packs<T, N, PART_PACKS>(f, v);
+            f = reduce<256>(f, sm[turn]);
+            turn ^= 1;
+            if (tid == 0) soft[item] = f;
+        } else {
+            const long long a64 = p.actions[row];
+            const bool valid = a64 >= 0 && a64 < p.classes;
+            const float za = tid == 0 && valid ? (float)z[a64] : 0.f;
+            for (int i = tid; i < parts; i += 256) {
+                const Soft o = soft[row * parts + i];
+                const float m = fmaxf(f.m, o.m), m0 = finite_or_0(m);
+                f.s = f.s * exp_of(f.m, m0) + o.s * exp_of(o.m, m0);
+                f.m = m;
+            }
+            f = reduce<256>(f, sm[turn]);
+            if (tid == 0) {
+                double add[3] = {0.0, 0.0, 0.0};
+                coef_s[turn] = row_scalars(p, row, f, za, valid, count, add, part == 0);
+                if (part == 0)
+                    for (int k = 0; k < 3; ++k) sums[k] += add[k];
+            }
+            __syncthreads();
+            const float coef = coef_s[turn];
+            turn ^= 1;
+            if (!g) continue;
+            const float scale = -coef / f.s;
+#pragma unroll
+            for (int i = 0; i < PART_PACKS; ++i) own.store(g + c0, i, gradient_of<T, N>(v[i], f.m, scale));
+            // the thread that wrote the action's element writes it once more
+            const long long at = a64 - c0;
+            if (valid && at >= 0 && at < own.cols && tid == (int)at / N % 256) g[a64] = (T)(exp_of((float)z[a64], f.m) * scale + coef);
+        }
+    }
+    if (GRAD && !p.upstream) block_sums<256>(p.part, sums);
 }
 
 __global__ __launch_bounds__(1024) void policy_count_kernel(const unsigned char* __restrict__ mask, double* count,
@@ -340,7 +389,7 @@ __global__ __launch_bounds__(256) void policy_finish_kernel(const double* __rest
 }
 
 struct Plan {
-    int g, nv, vec;                                          // nv 0: too long for the registers of 1024 threads
+    int g, nv, vec;                                          // g 0: too long for the registers of 1024 threads
 };
 // The fewest threads whose registers hold the row: few waves wait for each other, more rows are in a CU at a time, and the rows
 // of a wave share the time of their scalars (65536 x 1000 bf16: 71 us with a wave a row).  Rows shorter than a pack are read by
@@ -354,7 +403,13 @@ Plan plan(int classes, int dtype) {
             const int nv = (packs + g - 1) / g;
             return Plan{g, nv <= 4 ? nv : (nv + 1) / 2 * 2, n};
         }
-    return Plan{1024, 0, n};
+    return Plan{0, 0, n};
+}
+// parts of a long row, and columns of a part (whole packs)
+int parts_of(int classes, int vec, int& span) {
+    const int packs = (classes - 1) / vec + 1, parts = (packs - 1) / (256 * PART_PACKS) + 1;
+    span = ((packs - 1) / parts + 1) * vec;
+    return (classes - 1) / span + 1;
 }
 int blocks_of(long long rows, const Plan& p) {
     const int rpb = p.g < 256 ? 256 / p.g : 1, cap = p.g == 1024 ? 512 : p.g == 512 ? 1024 : MAX_BLOCKS;
@@ -376,14 +431,22 @@ void launch(const Plan& pl, int blocks, const Args& a, hipStream_t st) {
     else if (pl.g == 64) launch_nv<T, N, 64, 3, 16>(pl.nv, blocks, a, st);
     else if (pl.g == 256) launch_nv<T, N, 256, 6, 16>(pl.nv, blocks, a, st);
     else if (pl.g == 512) launch_nv<T, N, 512, 10, 16>(pl.nv, blocks, a, st);
-    else if (pl.nv) launch_nv<T, N, 1024, 10, 16>(pl.nv, blocks, a, st);
-    else hipLaunchKernelGGL((policy_kernel<T, N, 0, 1, 1024>), dim3(blocks), dim3(1024), 0, st, a);
+    else launch_nv<T, N, 1024, 10, 16>(pl.nv, blocks, a, st);
+}
+template <typename T>
+void launch_parts(int parts, int span, int blocks, const Args& a, Soft* soft, hipStream_t st) {
+    constexpr int N = 16 / (int)sizeof(T);
+    if (!a.upstream) hipLaunchKernelGGL((policy_parts_kernel<T, N, false>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
+    hipLaunchKernelGGL((policy_parts_kernel<T, N, true>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
 }
 
 }  // namespace
 
-extern "C" size_t step_policy_loss_ws_bytes(long long rows) {
-    return rows > 0 ? (1 + 3 * (size_t)MAX_BLOCKS) * sizeof(double) : 0;
+extern "C" size_t step_policy_loss_ws_bytes(long long rows, int classes) {
+    if (rows <= 0 || classes <= 0 || classes > 1 << 30) return 0;
+    int span;                                                // (fp32's parts: a 16-bit type has fewer)
+    const size_t soft = plan(classes, STEP_F32).g ? 0 : (size_t)rows * parts_of(classes, 4, span) * sizeof(Soft);
+    return (1 + 3 * (size_t)MAX_BLOCKS) * sizeof(double) + soft;
 }
 
 extern "C" int step_policy_loss(const void* logits, const long long* actions, const float* old_logp,
@@ -396,21 +459,32 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
     STEP_REQUIRE(elem_bytes(dtype), "step_policy_loss: unknown type %d", dtype);
     STEP_REQUIRE(upstream ? dlogits != nullptr : loss && stats && logp, "step_policy_loss: null output");
     STEP_REQUIRE((((uintptr_t)logits | (uintptr_t)dlogits) & (elem_bytes(dtype) - 1)) == 0, "step_policy_loss: logits or dlogits lie across elements");
-    if (ws_bytes < step_policy_loss_ws_bytes(rows)) {
-        step::set_error("step_policy_loss: workspace %zu < %zu bytes", ws_bytes, step_policy_loss_ws_bytes(rows));
+    if (ws_bytes < step_policy_loss_ws_bytes(rows, classes)) {
+        step::set_error("step_policy_loss: workspace %zu < %zu bytes", ws_bytes, step_policy_loss_ws_bytes(rows, classes));
         return STEP_ERR_WORKSPACE;
     }
     hipStream_t st = (hipStream_t)stream;
     double* count = (double*)ws;
     double* part = count + 1;
     const Plan pl = plan(classes, dtype);
-    const int blocks = blocks_of(rows, pl);
+    int blocks, parts = 0, span = 0;
+    if (pl.g) {
+        blocks = blocks_of(rows, pl);
+    } else {
+        parts = parts_of(classes, pl.vec, span);
+        blocks = rows * parts < MAX_BLOCKS ? (int)(rows * parts) : MAX_BLOCKS;
+    }
     if (mask && !upstream) hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(1024), 0, st, mask, count, rows);
     const Args a{logits, actions, old_logp, advantages, ref_logp, mask, dlogits, logp, mask ? count : nullptr, part,
                  upstream, skip_one, rows, classes, clip_low, clip_high, beta};
-    if (dtype == STEP_F32) launch<float>(pl, blocks, a, st);
-    else if (dtype == STEP_BF16) launch<bf16>(pl, blocks, a, st);
-    else launch<f16>(pl, blocks, a, st);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        if (pl.g) launch<T>(pl, blocks, a, st);
+        else launch_parts<T>(parts, span, blocks, a, (Soft*)(part + 3 * MAX_BLOCKS), st);
+    };
+    if (dtype == STEP_F32) go(float());
+    else if (dtype == STEP_BF16) go(bf16());
+    else go(f16());
     if (!upstream)
         hipLaunchKernelGGL(policy_finish_kernel, dim3(1), dim3(256), 0, st, part, mask ? count : nullptr, (double)rows,
                            blocks, beta, loss, stats);

@@ -81,7 +81,7 @@ class _PolicyLossFn(torch.autograd.Function):
         grad = torch.empty_like(z) if need else None
         ctx.mark_non_differentiable(logp, stats)
         ctx.config = (clip_low, clip_high, beta)
-        nb = _lib.size("step_policy_loss_ws_bytes", rows)
+        nb = _lib.size("step_policy_loss_ws_bytes", rows, classes)
         ws = z.new_empty(nb, dtype=torch.uint8)
         if not rows:
             loss.zero_(), stats.zero_()

@@ -121,7 +121,7 @@ def test_layer_norm_abi():
 
 
 def test_policy_loss_abi():
-    nb = _lib.query("step_policy_loss_ws_bytes", 4)
+    nb = _lib.query("step_policy_loss_ws_bytes", 4, 8)
     ok = (PTR, PTR, PTR, PTR, None, None, 0.2, 0.2, 0.0, None, 0, PTR, PTR, PTR, PTR, 4, 8, 0, PTR, nb, None)
     for i, bad, rcode in ((0, None, -1), (1, None, -1), (2, None, -1), (3, None, -1), (11, None, -1), (12, None, -1), (13, None, -1), (15, 0, -1),
                           (16, 0, -1), (17, 9, -1), (18, None, -1), (19, nb - 1, -3), (14, ctypes.c_void_p(4098), -1), (0, ctypes.c_void_p(4098), -1)):
