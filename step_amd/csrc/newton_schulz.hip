@@ -8,14 +8,19 @@
 // r <= 64, all in fp64: X_k = P_k X_0 with P_k and A_k polynomials of A_0, so the long side is read twice only - once for
 //   G G^T and once for P G: A <- q(A) A q(A), P <- q(A) P, r x r products on the fp64 matrix cores.  The recursion on A
 //   multiplies a small eigenvalue's error by up to a^2 in every step, which fp32 does not bear and fp64 does.
-//   The trace of G G^T is the squared norm.  Three launches for a whole list of matrices: bound by latency.
+//   The trace of G G^T is the squared norm.  Three launches for a whole list of matrices: bound by the latency of a chain of
+//   16 x 16 x 4 fp64 products (64 cycles each) on one CU a matrix.  The matrices of a classifier of widths 32, 64, 64 with 75
+//   taps (14 MB with momentum and update): 14 + 47 + 16 us; 7.6 us of the second launch a step at r = 64.
 //
 // r > 64, every product on the f16 matrix cores: a value v, scaled by a power of two, is hi = f16(v) plus lo = f16(v - hi)
 //   (together 22 bits and the sign of lo: the 24 bits of an fp32 value to half a unit or so), a product takes three terms
 //   hi hi + hi lo + lo hi with fp32 accumulation.  The dropped lo lo is 2^-24 of a product.  The singular values stay
 //   under 1.21 (q's maximum on [0, 1.46]) and so do all elements, so the scales are constants.  Matrices lie packed, 32
 //   hi and 32 lo of a row in 128 bytes, X also transposed, so that every product has both its operands along the
-//   contraction.  A and q(A) are symmetric: only the tiles on and over the diagonal are computed.
+//   contraction.  A and q(A) are symmetric: only the tiles on and over the diagonal are computed.  Bound by the matrix cores where
+//   the products fill the card (4096 x 4096: X's update 350 us, 1.18 PFLOP/s of f16 products, the cores busy in 65 % of the
+//   cycles at the 1.8 GHz that their power leaves; a plain f16 product of 8192^3 reaches 1.02), by the chain of r x r products
+//   otherwise (256 x 19200: 28 of them, 6 us each).  A value under 2^-28 of the norm keeps fewer bits: its error is 2^-39.
 #include <vector>
 #include "rows.h"
 
@@ -165,13 +170,23 @@ __global__ __launch_bounds__(64 * GRAM_WAVES) void ns_gram_kernel(const SmallArg
     for (int e = threadIdx.x; e < 2560; e += 64 * GRAM_WAVES) slab[e] = (sm[0][e] + sm[1][e]) + (sm[2][e] + sm[3][e]);
 }
 
-// C = X Y for commuting symmetric X, Y of 16 NT rows in LDS: one tile on or over the diagonal a wave, mirrored; f(i, j, value) stores
-template <int NT, typename F>
-__device__ __forceinline__ void sym_product(const double* X, const double* Y, F f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
-    if (wave >= NT * (NT + 1) / 2) return;
-    int a = 0, b = wave;
-    while (b >= NT) b -= NT - ++a;                           // row a of the triangle has NT - a tiles
+// Products X Y of commuting symmetric matrices of 16 NT rows in LDS, by 16 x 16 tiles on or over the diagonal, a wave each.
+constexpr int SMALL_THREADS = 1024;
+template <int NT>
+constexpr int tri_of() {
+    return NT * (NT + 1) / 2;
+}
+template <int NT>
+__device__ __forceinline__ void tile_at(int t, int& a, int& b) {   // row a of the triangle has NT - a tiles
+    a = 0;
+    b = t;
+    while (b >= NT) b -= NT - ++a;
+}
+template <int NT>
+__device__ __forceinline__ f64x4 sym_tile(const double* X, const double* Y, int tile) {
+    const int lane = threadIdx.x & 63, i16 = lane & 15, q = lane >> 4;
+    int a, b;
+    tile_at<NT>(tile, a, b);
     const double* x = X + (16 * a + i16) * S_P + q;
     const double* y = Y + (16 * b + i16) * S_P + q;
     f64x4 c{0, 0, 0, 0}, d{0, 0, 0, 0};
@@ -180,39 +195,53 @@ __device__ __forceinline__ void sym_product(const double* X, const double* Y, F 
         c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * s], y[4 * s], c, 0, 0, 0);
         d = __builtin_amdgcn_mfma_f64_16x16x4f64(x[4 * s + 4], y[4 * s + 4], d, 0, 0, 0);
     }
+    return c + d;
+}
+// a tile and its mirror image: f(i, j, value) stores, one value for both places, bit for bit
+template <int NT, typename F>
+__device__ __forceinline__ void mirrored(const f64x4& v, int tile, F f) {
+    const int lane = threadIdx.x & 63, i16 = lane & 15, q = lane >> 4;
+    int a, b;
+    tile_at<NT>(tile, a, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int row = 16 * a + 4 * i + q, col = 16 * b + i16;
-        const double v = c[i] + d[i];
-        if (a != b || row <= col) {                          // one value for both places, bit for bit
-            f(row, col, v);
-            if (row != col) f(col, row, v);
+        if (a != b || row <= col) {
+            f(row, col, v[i]);
+            if (row != col) f(col, row, v[i]);
         }
     }
 }
-constexpr int SMALL_THREADS = 640;                           // ten tiles of 16 x 16
 
-// A in LDS (its trace in `tr`) -> P with O = P G
+// A in LDS -> P with O = P G.  A step is three rounds of products: Q = q(A) from A^2; Q P and Q A, whose tiles (20 at r = 64) are
+// five for each SIMD; (Q A) Q.  Results take their operand's place once all waves have read it.
 template <int NT>
-__device__ __forceinline__ void small_steps(double* A, double* Q, double*& P, double* W, double inv, int steps) {
+__device__ __forceinline__ void small_steps(double* A, double* Q, double* P, double inv, int steps) {
+    constexpr int T = tri_of<NT>(), WAVES = SMALL_THREADS / 64;
+    const int wave = threadIdx.x >> 6;
+    auto into = [](double* M) { return [M](int i, int j, double v) { M[i * S_P + j] = v; }; };
     for (int step = 0; step < steps; ++step) {
-        sym_product<NT>(A, A, [&](int i, int j, double v) {
-            const double w = QB * A[i * S_P + j] + QC * v + (i == j ? QA : 0.0);
-            Q[i * S_P + j] = w;
-            if (step == 0) P[i * S_P + j] = w * inv;
-        });
+        if (wave < T)
+            mirrored<NT>(sym_tile<NT>(A, A, wave), wave, [&](int i, int j, double v) {
+                const double w = QB * A[i * S_P + j] + QC * v + (i == j ? QA : 0.0);
+                Q[i * S_P + j] = w;
+                if (step == 0) P[i * S_P + j] = w * inv;
+            });
         __syncthreads();
-        if (step) {
-            sym_product<NT>(Q, P, [&](int i, int j, double v) { W[i * S_P + j] = v; });
-            __syncthreads();
-            double* t = P;
-            P = W;
-            W = t;
-        }
+        // tiles [0, T) of Q P (not in the first step), [T, 2 T) of Q A (not in the last)
+        const int from = step ? 0 : T, to = step + 1 < steps ? 2 * T : T;
+        const int u0 = from + wave, u1 = u0 + WAVES;
+        f64x4 v0, v1;
+        if (u0 < to) v0 = sym_tile<NT>(Q, u0 < T ? P : A, u0 < T ? u0 : u0 - T);
+        if (u1 < to) v1 = sym_tile<NT>(Q, u1 < T ? P : A, u1 < T ? u1 : u1 - T);
+        __syncthreads();
+        if (u0 < to) mirrored<NT>(v0, u0 < T ? u0 : u0 - T, into(u0 < T ? P : A));
+        if (u1 < to) mirrored<NT>(v1, u1 < T ? u1 : u1 - T, into(u1 < T ? P : A));
+        __syncthreads();
         if (step + 1 < steps) {
-            sym_product<NT>(Q, A, [&](int i, int j, double v) { W[i * S_P + j] = v; });
+            if (wave < T) v0 = sym_tile<NT>(A, Q, wave);
             __syncthreads();
-            sym_product<NT>(W, Q, [&](int i, int j, double v) { A[i * S_P + j] = v; });
+            if (wave < T) mirrored<NT>(v0, wave, into(A));
             __syncthreads();
         }
     }
@@ -224,17 +253,19 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const SmallArgs
     int local;
     const SmallItem& it = find(p, blockIdx.x, local);
     const int r = min(it.m, it.n), nt = (r + 15) / 16, R = 16 * nt, tid = threadIdx.x;
-    double *A = lds, *Q = lds + 64 * S_P, *P = lds + 2 * 64 * S_P, *W = lds + 3 * 64 * S_P;
+    double *A = lds, *Q = lds + 64 * S_P, *P = lds + 2 * 64 * S_P;
     const double* slab = p.ws + it.slab + (size_t)local * it.chunks * 2560;
     // join the chunks in order: element e of tile t is row 16 a + 4 (e / 64) + (e % 64) / 16, column 16 b + e % 16
-    double v[4] = {0.0, 0.0, 0.0, 0.0};
+    constexpr int NJ = (2560 + SMALL_THREADS - 1) / SMALL_THREADS;
+    double v[NJ] = {};
 #pragma unroll 8
     for (int c = 0; c < it.chunks; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += slab[(size_t)c * 2560 + tid + SMALL_THREADS * j];
+        for (int j = 0; j < NJ; ++j) v[j] += slab[(size_t)c * 2560 + min(tid + SMALL_THREADS * j, 2559)];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < NJ; ++j) {
         const int e = tid + SMALL_THREADS * j;
+        if (e >= 2560) continue;
         const int t = e >> 8, a = t < 4 ? 0 : t < 7 ? 1 : t < 9 ? 2 : 3, b = t < 4 ? t : t < 7 ? t - 3 : t < 9 ? t - 5 : 3;
         const int row = 16 * a + 4 * ((e & 255) >> 6) + ((e & 63) >> 4), col = 16 * b + (e & 15);
         if (b >= nt || (a == b && row > col)) continue;
@@ -251,10 +282,10 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const SmallArgs
     const double inv = norm_s;
     for (int e = tid; e < 64 * R; e += SMALL_THREADS) A[(e >> 6) * S_P + (e & 63)] *= inv * inv;
     __syncthreads();
-    if (nt == 1) small_steps<1>(A, Q, P, W, inv, p.steps);
-    else if (nt == 2) small_steps<2>(A, Q, P, W, inv, p.steps);
-    else if (nt == 3) small_steps<3>(A, Q, P, W, inv, p.steps);
-    else small_steps<4>(A, Q, P, W, inv, p.steps);
+    if (nt == 1) small_steps<1>(A, Q, P, inv, p.steps);
+    else if (nt == 2) small_steps<2>(A, Q, P, inv, p.steps);
+    else if (nt == 3) small_steps<3>(A, Q, P, inv, p.steps);
+    else small_steps<4>(A, Q, P, inv, p.steps);
     double* out = p.ws + it.p + (size_t)local * 4096;
     for (int e = tid; e < 64 * R; e += SMALL_THREADS)
         if ((e & 63) < R) out[e] = P[(e >> 6) * S_P + (e & 63)];
@@ -268,7 +299,7 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const SmallArgs p) {
     int local;
     const SmallItem& it = find(p, z, local);
     const bool tall = it.m > it.n;
-    const int r = tall ? it.n : it.m, l = tall ? it.m : it.n, nt = (r + 15) / 16, R = 16 * nt;
+    const int r = tall ? it.n : it.m, l = tall ? it.m : it.n, nt = (r + 15) / 16;
     if (part * 64 >= l) return;
     const Io io = shifted(it.io, (size_t)local * it.m * it.n, sizeof(T));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
@@ -296,8 +327,11 @@ __global__ __launch_bounds__(256) void ns_apply_kernel(const SmallArgs p) {
             size_t at;
             old[a][i] = place(a, i, at) && io.param ? io.param[at] : 0.f;
         }
-    for (int e = threadIdx.x; e < 64 * R; e += 256)
-        if ((e & 63) < R) P[(e >> 6) * S_P + (e & 63)] = src[e];
+    double pv[16];                                           // all 64 x 64, of which 16 nt rows and columns are looked at
+#pragma unroll
+    for (int k = 0; k < 16; ++k) pv[k] = src[threadIdx.x + 256 * k];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) P[(4 * k + (threadIdx.x >> 6)) * S_P + (threadIdx.x & 63)] = pv[k];
     __syncthreads();
     if (c0 >= l) return;
 #pragma unroll
@@ -469,11 +503,11 @@ constexpr int stages_of() {
 }
 // acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 64 NT) of B over the stages [s0, s1): operands packed alike, K along both.
 // A stage lies in LDS as rows of 128 bytes whose eight 16-byte pieces are in the order piece ^ order(row): 16 neighbouring rows
-// are read from different banks (64 banks hold two rows).  Three stages in LDS, copied there directly, two of them in flight.  A wave reads the
-// operands of the next half stage before it multiplies the present one; one barrier a stage, in the middle: before it a
-// wave has its reads of the stage behind it and its copies of the next one, after it the stage's place is filled again.
-// The tile is what LDS reads allow: 192 rows read per 128 x 64 x 3 products keep the matrix cores ahead of LDS (94 of 128
-// bytes a cycle); 64 x 64 a wave needs 125.
+// are read from different banks (64 banks hold two rows).  Three to six stages in LDS, copied there directly, all but one in
+// flight.  A wave reads the operands of the next half stage among the products of the present one; one barrier a stage, in the
+// middle: before it a wave has its reads of the stage behind it and its copies of the next one, after it the stage's place is
+// filled again.  A wave's 128 x 64 reads 192 rows for three products of 128 x 64: 94 of the 128 bytes that LDS gives a cycle; with
+// 64 x 64 it is 125, with 32 x 32 LDS bounds (950 cycles a stage for half, 420 for an eighth of the products of 1600).
 template <int MT>
 __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
     constexpr int NT = nt_of<MT>(), TM = 64 * MT, TN = 64 * NT, STAGE = (TM + TN) * ROWB, NST = stages_of<MT>();
@@ -817,10 +851,11 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, in
 struct Share {
     int mt, tiles, full, rest, splits;
 };
-// The variant that takes the least time by this count, in cycles: a stage takes 1536 on the matrix cores at 256 x 128 a tile, half of it
-// at 128 x 128 (1600 and 850 were measured, with the waits); a tile's beginning and end 8000; writing and joining the parts
-// of split tiles 26000 (9 us over 16 tiles, 14 us over 75).  4096 x 4096: 272 tiles of 256 x 128 as 256 and 16 x 16 parts;
-// three stacked 1152 x 1152: 135 tiles of 128 x 128 at once (19 us) and not 75 x 3 parts of 256 x 128 (26 + 12 us).
+// The variant that takes the least time by this count, in cycles, as measured: a stage 1600 at 256 x 128 a tile (1536 of them on the
+// matrix cores), 950 at 128 x 128, 420 at 64 x 64; a tile's beginning and end 12000, or 7000; writing and joining the parts of
+// split tiles 26000.  Both sides of some choices: 4096 x 4096 as 256 tiles of 256 x 128 and 16 x 16 parts 194 + 9 us, as 272 tiles
+// 354; three stacked 1152 x 1152 as 135 tiles of 128 x 128 27 us, as 75 x 3 parts of 256 x 128 26 + 12; 512 x 512 by 64 x 64
+// tiles all five steps 140 us, by 128 x 128 250; 256 x 19200 183 and 263.
 Share share(int mt, long long tiles, long long total) {
     Share s{mt, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
     return s;
@@ -887,7 +922,8 @@ Layout layout(int batch, int m, int n) {
     o.xt2 = take(sub * R * L * 4);
     // steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
     // products of r x r matrices, of which each further step takes three more.  Worth it where X is longer than wide (by count at
-    // l > r; from l = 2 r it also outweighs that r x r products fill the card less).  An error of A grows by a^2 = 12 in each
+    // l > r; from l = 2 r it also outweighs that r x r products fill the card less: 3 x 4101 x 1030 1020 -> 813 us, 256 x 19200
+    // 294 -> 263 when it was taken).  An error of A grows by a^2 = 12 in each
     // step of a group for the smallest eigenvalues: three fp32-accurate steps cost them 2e-5 of the largest, less than what
     // X X^T over that length is off by.
     o.group = l >= 2 * r ? 3 : 1;
@@ -1075,7 +1111,7 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
         std::vector<SmallItem> sm;
         std::vector<int> firsts;
         small_groups(items, idx, groups, sm, firsts);
-        constexpr size_t lds = 4 * 64 * S_P * sizeof(double);
+        constexpr size_t lds = 3 * 64 * S_P * sizeof(double);
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ns_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) {
             step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
