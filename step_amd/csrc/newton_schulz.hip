@@ -851,18 +851,17 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, in
 struct Share {
     int mt, tiles, full, rest, splits;
 };
-// The variant that takes the least time by this count, in cycles, as measured: a stage 1600 at 256 x 128 a tile (1536 of them on the
-// matrix cores), 950 at 128 x 128, 420 at 64 x 64; a tile's beginning and end 12000, or 7000; writing and joining the parts of
-// split tiles 26000.  Both sides of some choices: 4096 x 4096 as 256 tiles of 256 x 128 and 16 x 16 parts 194 + 9 us, as 272 tiles
-// 354; three stacked 1152 x 1152 as 135 tiles of 128 x 128 27 us, as 75 x 3 parts of 256 x 128 26 + 12; 512 x 512 by 64 x 64
-// tiles all five steps 140 us, by 128 x 128 250; 256 x 19200 183 and 263.
+// The variant that takes the least time by this count, in cycles at the 1.8 GHz of a full card: a stage 2290 at 256 x 128 a tile (1536
+// of them on the matrix cores), 1150 at 128 x 128, 480 at 64 x 64; a tile's beginning and end; writing the parts of split tiles
+// and joining them.  All five steps in us, as chosen / tiles never split / 128 x 128 at least / 256 x 128 only: 4096 x 4096 fp32
+// 3705 / 4160 / 3705 / 3705, 256 x 19200 180 / 389 / 260 / 377, 512 x 512 136 / 136 / 234 / 406, 1024 x 4096 296 / 326 / 457 / 506.
 Share share(int mt, long long tiles, long long total) {
     Share s{mt, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
     return s;
 }
 double cycles(const Share& s, int stages) {
-    const double one = s.mt == 4 ? 1600 : s.mt == 2 ? 950 : 420, ends = s.mt == 1 ? 7000 : 12000, round = stages * one + ends;
-    return s.full / CUS * round + (s.rest ? (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + ends + 26000 : round) : 0);
+    const double one = s.mt == 4 ? 2290 : s.mt == 2 ? 1150 : 480, ends = s.mt == 4 ? 18000 : s.mt == 2 ? 11000 : 7000, round = stages * one + ends;
+    return s.full / CUS * round + (s.rest ? (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + ends + 12000 + 150 * s.rest : round) : 0);
 }
 Share best(const Share& a, const Share& b, int stages) { return cycles(b, stages) < cycles(a, stages) ? b : a; }
 Share fastest(int mt, long long tiles, int nb, int stages) {
@@ -920,13 +919,13 @@ Layout layout(int batch, int m, int n) {
     o.x = take(sub * RA * L * 4);
     o.xt = take(sub * R * L * 4);
     o.xt2 = take(sub * R * L * 4);
-    // steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
-    // products of r x r matrices, of which each further step takes three more.  Worth it where X is longer than wide (by count at
-    // l > r; from l = 2 r it also outweighs that r x r products fill the card less: 3 x 4101 x 1030 1020 -> 813 us, 256 x 19200
-    // 294 -> 263 when it was taken).  An error of A grows by a^2 = 12 in each
-    // step of a group for the smallest eigenvalues: three fp32-accurate steps cost them 2e-5 of the largest, less than what
-    // X X^T over that length is off by.
-    o.group = l >= 2 * r ? 3 : 1;
+    // Steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
+    // products of r x r matrices, of which each further step takes three more: where the two passes over X cost more than those
+    // (256 x 19200: 180 us, 237 step by step; 3 x 4101 x 1030 765 and 1047; 400 x 900, taken step by step, 145, and 156 together).
+    // An error of A grows by a^2 = 12 in each step of a group for the smallest eigenvalues: three fp32-accurate steps cost them
+    // 2e-5 of the largest, less than what X X^T over a length of 2 r is off by.
+    const double passes = cycles(o.xxt, step::ceil_div(l, KS)) + cycles(o.update, step::ceil_div(r, KS));
+    o.group = l >= 2 * r && passes > 3 * cycles(o.sym, step::ceil_div(r, KS)) ? 3 : 1;
     for (int i = 0; i < (o.group > 1 ? 4 : 2); ++i) o.r[i] = take(sub * RA * R * 4);
     // shares of split tiles: fewer than one a CU, of 256 x 128 at most.  A last part of the batch that is smaller is shared out anew.
     const bool any = sub < batch || o.xxt.splits > 1 || o.sym.splits > 1 || o.update.splits > 1;
