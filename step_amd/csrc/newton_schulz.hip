@@ -18,9 +18,9 @@
 //   under 1.21 (q's maximum on [0, 1.46]) and so do all elements, so the scales are constants.  Matrices lie packed, 32
 //   hi and 32 lo of a row in 128 bytes, X also transposed, so that every product has both its operands along the
 //   contraction.  A and q(A) are symmetric: only the tiles on and over the diagonal are computed.  Bound by the matrix cores where
-//   the products fill the card (4096 x 4096: X's update 350 us, 1.18 PFLOP/s of f16 products, the cores busy in 65 % of the
+//   the products fill the card (4096 x 4096: X's update 355 us, 1.16 PFLOP/s of f16 products, the cores busy in 65 % of the
 //   cycles at the 1.8 GHz that their power leaves; a plain f16 product of 8192^3 reaches 1.02), by the chain of r x r products
-//   otherwise (256 x 19200: 28 of them, 6 us each).  A value under 2^-28 of the norm keeps fewer bits: its error is 2^-39.
+//   otherwise (256 x 19200: 14 of them, 6 us each, of 176).  A value under 2^-28 of the norm keeps fewer bits: its error is 2^-39.
 #include <vector>
 #include "rows.h"
 
@@ -465,24 +465,24 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     }
 }
 
-// Tiles: 64 MT x 64 NT, a wave's share 32 MT x 32 NT.  MT = 4 and 2 have NT = 2, MT = 1 has 1 (for products too small to fill the CUs).
-template <int MT>
-constexpr int nt_of() {
-    return MT == 1 ? 1 : 2;
-}
+// Tiles: 64 MT x 64 NT, a wave's share 32 MT x 32 NT.  The variants V: 0 is 256 x 128, 1 128 x 128, 2 128 x 64 and 3 64 x 64, for
+// products too small to fill the CUs with larger ones.
+constexpr int VARIANTS = 4;
+constexpr int mt_of(int v) { return v == 0 ? 4 : v == 3 ? 1 : 2; }
+constexpr int nt_of(int v) { return v < 2 ? 2 : 1; }
 // The products of the hi parts, and the two small terms in sums of their own, so that the large sum is rounded once per product
 // and not three times.
-template <int MT>
+template <int V>
 struct Acc {
-    f32x16 v[MT][nt_of<MT>()], w[MT][nt_of<MT>()];
+    f32x16 v[mt_of(V)][nt_of(V)], w[mt_of(V)][nt_of(V)];
 };
-template <int MT>
+template <int V>
 struct Frag {
-    f16x8 ah[MT], al[MT], bh[nt_of<MT>()], bl[nt_of<MT>()];
+    f16x8 ah[mt_of(V)], al[mt_of(V)], bh[nt_of(V)], bl[nt_of(V)];
 };
-template <int MT>
-__device__ __forceinline__ void multiply(Acc<MT>& acc, const Frag<MT>& f) {
-    constexpr int NT = nt_of<MT>();
+template <int V>
+__device__ __forceinline__ void multiply(Acc<V>& acc, const Frag<V>& f) {
+    constexpr int MT = mt_of(V), NT = nt_of(V);
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -497,21 +497,22 @@ __device__ __forceinline__ void multiply(Acc<MT>& acc, const Frag<MT>& f) {
         for (int b = 0; b < NT; ++b) acc.w[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[a], f.bl[b], acc.w[a][b], 0, 0, 0);
 }
 
-template <int MT>
+template <int V>
 constexpr int stages_of() {
-    return MT == 4 ? 3 : MT == 2 ? 4 : 6;
+    return V == 0 ? 3 : V == 2 ? 3 : 4;
 }
 // acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 64 NT) of B over the stages [s0, s1): operands packed alike, K along both.
 // A stage lies in LDS as rows of 128 bytes whose eight 16-byte pieces are in the order piece ^ order(row): 16 neighbouring rows
-// are read from different banks (64 banks hold two rows).  Three to six stages in LDS, copied there directly, all but one in
+// are read from different banks (64 banks hold two rows).  Three or four stages in LDS, copied there directly, all but one in
 // flight.  A wave reads the operands of the next half stage among the products of the present one; one barrier a stage, in the
 // middle: before it a wave has its reads of the stage behind it and its copies of the next one, after it the stage's place is
 // filled again.  A wave's 128 x 64 reads 192 rows for three products of 128 x 64: 94 of the 128 bytes that LDS gives a cycle; with
-// 64 x 64 it is 125, with 32 x 32 LDS bounds (950 cycles a stage for half, 420 for an eighth of the products of 1600).
-template <int MT>
-__device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
-    constexpr int NT = nt_of<MT>(), TM = 64 * MT, TN = 64 * NT, STAGE = (TM + TN) * ROWB, NST = stages_of<MT>();
+// 64 x 64 it is 125, with less LDS bounds.  The smaller two variants' stages leave room for a second tile in a CU.
+template <int V>
+__device__ __forceinline__ void main_loop(Acc<V>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
+    constexpr int MT = mt_of(V), NT = nt_of(V), TM = 64 * MT, TN = 64 * NT, STAGE = (TM + TN) * ROWB, NST = stages_of<V>();
     constexpr int NA = TM / 32, NB = TN / 32, NL = NA + NB;                  // a wave's copies, of 8 rows each
+    constexpr int GROUPS = V == 0 ? 12 : V == 1 ? 4 : V == 2 ? 3 : 1;        // reads are issued in so many parts, a product between two
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, q = lane >> 5;
     const size_t pitch = (size_t)(K / KS) * ROWB;
     const int lrow = lane >> 3, piece = (lane & 7) ^ lrow, order = (l31 & 7) ^ ((l31 >> 3) & 1);
@@ -535,7 +536,7 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
     };
     const char* ra = lds + ((wave >> 1) * (TM / 2) + l31) * ROWB;
     const char* rb = lds + (TM + (wave & 1) * (TN / 2) + l31) * ROWB;
-    auto read = [&](Frag<MT>& f, int buf, int kk) {
+    auto read = [&](Frag<V>& f, int buf, int kk) {
         const int hi = buf * STAGE + (((kk * 2 + q) ^ order) * 16), lo = buf * STAGE + (((4 + kk * 2 + q) ^ order) * 16);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -552,7 +553,7 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
     for (int i = 0; i < NST; ++i) issue(s0 + i, i);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * NL) : "memory");
     __builtin_amdgcn_s_barrier();
-    Frag<MT> f0, f1;
+    Frag<V> f0, f1;
     read(f0, 0, 0);
     int buf = 0;
     for (int s = s0; s < s1; ++s) {
@@ -563,8 +564,8 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
         multiply(acc, f0);
         // the reads among the first half of the products: the rest of them covers the last read's way
 #pragma unroll
-        for (int i = 0; i < (MT == 4 ? 12 : MT == 2 ? 4 : 1); ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, MT == 4 ? 1 : MT == 2 ? 2 : 4, 0);
+        for (int i = 0; i < GROUPS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * (MT + NT) / GROUPS, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -578,8 +579,8 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
         issue(s + NST, buf);
         multiply(acc, f1);
 #pragma unroll
-        for (int i = 0; i < (MT == 4 ? 12 : MT == 2 ? 4 : 1); ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, MT == 4 ? 1 : MT == 2 ? 2 : 4, 1);
+        for (int i = 0; i < GROUPS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * (MT + NT) / GROUPS, 1);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
         }
 #pragma unroll
@@ -595,10 +596,10 @@ __device__ __forceinline__ void main_loop(Acc<MT>& acc, const char* A, const cha
 }
 
 // f(row, column, value) for the wave's share of a tile
-template <int MT, typename F>
-__device__ __forceinline__ void each(const Acc<MT>& acc, F f) {
+template <int V, typename F>
+__device__ __forceinline__ void each(const Acc<V>& acc, F f) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, q = lane >> 5;
-    constexpr int NT = nt_of<MT>();
+    constexpr int MT = mt_of(V), NT = nt_of(V);
     const int wi = (wave >> 1) * 32 * MT, wj = (wave & 1) * 32 * NT;
 #pragma unroll
     for (int a = 0; a < MT; ++a)
@@ -619,9 +620,9 @@ __device__ __host__ __forceinline__ int tri_count(int cols, int per) {       // 
     for (int j = 0; j < cols; ++j) n += j / per + 1;
     return n;
 }
-template <int MT>
+template <int V>
 __device__ __forceinline__ void tri_tile(int t, int cols, int& ti, int& tj) {
-    constexpr int PER = MT / nt_of<MT>(), H = 8 / PER;   // columns of tiles per row of tiles; rows of tiles in a block
+    constexpr int PER = mt_of(V) / nt_of(V), H = 8 / PER;   // columns of tiles per row of tiles; rows of tiles in a block
     int J = 0;
     for (;; ++J) {
         const int w = cols - 8 * J < 8 ? cols - 8 * J : 8;
@@ -653,15 +654,15 @@ int tri_tiles(int cols, int per) {
     return n;
 }
 
-template <int PROD, int MT>
+template <int PROD, int V>
 __device__ __forceinline__ void locate(const Big& p, int tile, int& z, int& i0, int& j0, int tiles) {
-    constexpr int TN = 64 * nt_of<MT>();
+    constexpr int MT = mt_of(V), TN = 64 * nt_of(V);
     z = tile / tiles;
     int t = tile - z * tiles, ti, tj;
     if constexpr (PROD <= SYM) {
-        tri_tile<MT>(t, p.R / TN, ti, tj);
+        tri_tile<V>(t, (p.r + TN - 1) / TN, ti, tj);
     } else {                                       // eight columns of tiles at a time
-        const int rows = p.L / (64 * MT), cols = p.R / TN, g = t / (8 * rows), w = cols - 8 * g < 8 ? cols - 8 * g : 8, in = t - g * 8 * rows;
+        const int rows = (p.l + 64 * MT - 1) / (64 * MT), cols = (p.r + TN - 1) / TN, g = t / (8 * rows), w = cols - 8 * g < 8 ? cols - 8 * g : 8, in = t - g * 8 * rows;
         ti = in / w;
         tj = 8 * g + in % w;
     }
@@ -775,7 +776,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
 
 // Blocks [0, full): a tile each, the card's CUs filled `full / 256` times.  The tiles that are left share the card: `splits`
 // blocks a tile, each with a part of the contraction, whose sums ns_join_kernel adds up.
-template <int PROD, int MT, typename T>
+template <int PROD, int V, typename T>
 __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int tiles, int full, int splits) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     // blocks go to the eight XCDs in turn: each gets neighbouring tiles, whose operands its L2 then holds
@@ -789,7 +790,7 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
     }
     const bool whole = (int)blockIdx.x < full || splits == 1;
     int z, i0, j0;
-    locate<PROD, MT>(p, tile, z, i0, j0, tiles);
+    locate<PROD, V>(p, tile, z, i0, j0, tiles);
     const char *A, *B;
     int K;
     if constexpr (PROD == XXT) {
@@ -806,12 +807,12 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
     }
     const int stages = ((PROD == XXT ? p.l : p.r) + KS - 1) / KS;            // (behind them is nothing but zeros)
     const int s0 = whole ? 0 : (int)((long long)stages * split / splits), s1 = whole ? stages : (int)((long long)stages * (split + 1) / splits);
-    constexpr int TN = 64 * nt_of<MT>();
-    Acc<MT> acc;
+    constexpr int MT = mt_of(V), TN = 64 * nt_of(V);
+    Acc<V> acc;
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
-        for (int b = 0; b < nt_of<MT>(); ++b)
+        for (int b = 0; b < nt_of(V); ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[a][b][e] = acc.w[a][b][e] = 0.f;
     main_loop(acc, A, B, K, i0, j0, s0, s1, smem);
@@ -827,12 +828,12 @@ __global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int til
     }
 }
 // eight rows of a split tile, its shares added in order
-template <int PROD, int MT, typename T>
+template <int PROD, int V, typename T>
 __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, int full, int splits) {
-    constexpr int TN = 64 * nt_of<MT>(), EP = pitch_of<PROD, TN>();
+    constexpr int MT = mt_of(V), TN = 64 * nt_of(V), EP = pitch_of<PROD, TN>();
     __shared__ __attribute__((aligned(16))) float sm[8 * EP];
     int z, i0, j0;
-    locate<PROD, MT>(p, full + blockIdx.x, z, i0, j0, tiles);
+    locate<PROD, V>(p, full + blockIdx.x, z, i0, j0, tiles);
     const int i = threadIdx.x / (TN / 4), j = threadIdx.x % (TN / 4) * 4;
     if (i < 8) {
         const float* slab = p.slab + (size_t)blockIdx.x * splits * (64 * MT * TN) + (blockIdx.y * 8 + i) * TN + j;
@@ -847,25 +848,30 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, in
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// How a product's tiles are shared out: `mt` 32-row tiles a wave; whole rounds over the CUs, and the rest in `splits` parts
+// How a product's tiles are shared out: variant v; whole rounds over the CUs, and the rest in `splits` parts
 struct Share {
-    int mt, tiles, full, rest, splits;
+    int v, tiles, full, rest, splits;
 };
 // The variant that takes the least time by this count, in cycles at the 1.8 GHz of a full card: a stage 2290 at 256 x 128 a tile (1536
-// of them on the matrix cores), 1150 at 128 x 128, 480 at 64 x 64; a tile's beginning and end; writing the parts of split tiles
-// and joining them.  All five steps in us, as chosen / tiles never split / 128 x 128 at least / 256 x 128 only: 4096 x 4096 fp32
-// 3705 / 4160 / 3705 / 3705, 256 x 19200 180 / 389 / 260 / 377, 512 x 512 136 / 136 / 234 / 406, 1024 x 4096 296 / 326 / 457 / 506.
-Share share(int mt, long long tiles, long long total) {
-    Share s{mt, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
+// of them on the matrix cores), 1150 at 128 x 128, 690 at 128 x 64, 480 at 64 x 64; a tile's beginning and end, half of which two
+// small tiles in a CU share; writing the parts of split tiles and joining them.  All five steps in us, as chosen / tiles never split /
+// of 128 columns / of 256 x 128 only: 4096 x 4096 fp32 3655 / 4060 / 3657 / 3690, 256 x 19200 176 / 385 / 260 / 368, 512 x 512
+// 133 / 132 / 190 / 253, three stacked 4101 x 1030 bf16 682 / 689 / 761 / 895, 1024 x 4096 300 / 315 / 397 / 493.
+Share share(int v, long long tiles, long long total) {
+    Share s{v, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
     return s;
 }
 double cycles(const Share& s, int stages) {
-    const double one = s.mt == 4 ? 2290 : s.mt == 2 ? 1150 : 480, ends = s.mt == 4 ? 18000 : s.mt == 2 ? 11000 : 7000, round = stages * one + ends;
-    return s.full / CUS * round + (s.rest ? (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + ends + 12000 + 150 * s.rest : round) : 0);
+    static const double stage[VARIANTS] = {2290, 1150, 690, 480}, end[VARIANTS] = {18000, 11000, 14000, 7000};
+    const double one = stage[s.v], ends = end[s.v], more = s.v < 2 ? 1.0 : 0.5;   // (two small tiles are in a CU at a time)
+    const int rounds = s.full / CUS;
+    double c = rounds * stages * one + (rounds ? 1 + (rounds - 1) * more : 0) * ends;
+    if (s.rest) c += (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + ends + 12000 + 150 * s.rest : stages * one + (rounds ? more : 1) * ends);
+    return c;
 }
 Share best(const Share& a, const Share& b, int stages) { return cycles(b, stages) < cycles(a, stages) ? b : a; }
-Share fastest(int mt, long long tiles, int nb, int stages) {
-    Share s = share(mt, tiles, tiles * nb), t = s;
+Share fastest(int v, long long tiles, int nb, int stages) {
+    Share s = share(v, tiles, tiles * nb), t = s;
     if (s.rest) {
         t.splits = CUS / s.rest;
         if (t.splits > stages / 4) t.splits = stages / 4;
@@ -887,10 +893,10 @@ Layout layout_of(int nb, int r, int l) {
     const int sx = step::ceil_div(l, KS), sr = step::ceil_div(r, KS);
     auto of = [&](bool tri, int stages) {
         Share s{};
-        for (int mt : {4, 2, 1}) {
-            const int nt = mt == 1 ? 1 : 2, cols = o.R / (64 * nt);
-            const Share t = fastest(mt, tri ? tri_tiles(cols, mt / nt) : (long long)(o.L / (64 * mt)) * cols, nb, stages);
-            s = mt == 4 ? t : best(s, t, stages);
+        for (int v = 0; v < VARIANTS; ++v) {
+            const int mt = mt_of(v), nt = nt_of(v), cols = step::ceil_div(r, 64 * nt);
+            const Share t = fastest(v, tri ? tri_tiles(cols, mt / nt) : (long long)step::ceil_div(l, 64 * mt) * cols, nb, stages);
+            s = v == 0 ? t : best(s, t, stages);
         }
         return s;
     };
@@ -921,7 +927,7 @@ Layout layout(int batch, int m, int n) {
     o.xt2 = take(sub * R * L * 4);
     // Steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
     // products of r x r matrices, of which each further step takes three more: where the two passes over X cost more than those
-    // (256 x 19200: 180 us, 237 step by step; 3 x 4101 x 1030 765 and 1047; 400 x 900, taken step by step, 145, and 156 together).
+    // (256 x 19200: 176 us, 231 step by step; 3 x 4101 x 1030 682 and 956; 400 x 900, taken step by step, 141, and 150 together).
     // An error of A grows by a^2 = 12 in each step of a group for the smallest eigenvalues: three fp32-accurate steps cost them
     // 2e-5 of the largest, less than what X X^T over a length of 2 r is off by.
     const double passes = cycles(o.xxt, step::ceil_div(l, KS)) + cycles(o.update, step::ceil_div(r, KS));
@@ -1002,22 +1008,23 @@ int check(const step_ns_item* items, int count) {
     return STEP_OK;
 }
 
-template <int PROD, int MT, typename T>
+template <int PROD, int V, typename T>
 int product_of(const Big& p, const Share& s, hipStream_t st) {
-    auto kern = ns_product_kernel<PROD, MT, T>;
-    constexpr size_t lds = stages_of<MT>() * 64 * (MT + nt_of<MT>()) * ROWB;
+    auto kern = ns_product_kernel<PROD, V, T>;
+    constexpr size_t lds = stages_of<V>() * 64 * (mt_of(V) + nt_of(V)) * ROWB;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
         return STEP_ERR_LAUNCH;
     }
     hipLaunchKernelGGL(kern, dim3(s.full + s.rest * s.splits), dim3(256), lds, st, p, s.tiles, s.full, s.splits);
-    if (s.splits > 1) hipLaunchKernelGGL((ns_join_kernel<PROD, MT, T>), dim3(s.rest, 8 * MT), dim3(256), 0, st, p, s.tiles, s.full, s.splits);
+    if (s.splits > 1) hipLaunchKernelGGL((ns_join_kernel<PROD, V, T>), dim3(s.rest, 8 * mt_of(V)), dim3(256), 0, st, p, s.tiles, s.full, s.splits);
     return STEP_OK;
 }
 template <int PROD, typename T>
 int product(const Big& p, const Share& s, hipStream_t st) {
-    return s.mt == 4 ? product_of<PROD, 4, T>(p, s, st) : s.mt == 2 ? product_of<PROD, 2, T>(p, s, st) : product_of<PROD, 1, T>(p, s, st);
+    return s.v == 0 ? product_of<PROD, 0, T>(p, s, st) : s.v == 1 ? product_of<PROD, 1, T>(p, s, st) :
+           s.v == 2 ? product_of<PROD, 2, T>(p, s, st) : product_of<PROD, 3, T>(p, s, st);
 }
 template <typename T>
 int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
