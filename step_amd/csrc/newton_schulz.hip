@@ -70,7 +70,7 @@ struct SmallItem {
 struct SmallArgs {
     int first[S_ITEMS];                           // first matrix of each item; behind the items more than all
     SmallItem item[S_ITEMS];
-    int items, total, steps, max_chunks, max_parts;   // (parts: 64 columns each, of ns_apply_kernel)
+    int steps, max_chunks, max_parts;             // (parts: 64 columns each, of ns_apply_kernel)
     float eps;
     double* ws;
 };
@@ -947,7 +947,8 @@ struct Group {
     size_t doubles;
 };
 // small items in groups of one launch each; the workspace is used again by every group
-int small_groups(const step_ns_item* items, const std::vector<int>& idx, std::vector<Group>& groups, std::vector<SmallItem>& out, std::vector<int>& firsts) {
+void small_groups(const step_ns_item* items, const std::vector<int>& idx, std::vector<Group>& groups, std::vector<SmallItem>& out,
+                  std::vector<int>& firsts) {
     for (size_t i = 0; i < idx.size();) {
         Group g{(int)i, (int)i, 0, 1, 1, 0};
         int total = 0;
@@ -989,7 +990,6 @@ int small_groups(const step_ns_item* items, const std::vector<int>& idx, std::ve
         g.doubles = at;
         groups.push_back(g);
     }
-    return 0;
 }
 
 int check(const step_ns_item* items, int count) {
@@ -1125,15 +1125,14 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
         }
         for (const Group& g : groups) {
             SmallArgs a{};
-            a.items = g.end - g.begin;
-            a.total = g.total;
+            const int n = g.end - g.begin;
             a.steps = steps;
             a.max_chunks = g.max_chunks;
             a.max_parts = g.max_parts;
             a.eps = eps;
             a.ws = (double*)ws;
-            for (int i = 0; i < S_ITEMS; ++i) a.first[i] = i < a.items ? firsts[g.begin + i] : 0x7fffffff;
-            for (int i = 0; i < a.items; ++i) {
+            for (int i = 0; i < S_ITEMS; ++i) a.first[i] = i < n ? firsts[g.begin + i] : 0x7fffffff;
+            for (int i = 0; i < n; ++i) {
                 a.item[i] = sm[g.begin + i];
                 a.item[i].io = io_of(items[idx[g.begin + i]]);
             }

@@ -292,15 +292,15 @@ def test_inference_caches_see_a_step():
     assert torch.equal(after, want) and not torch.equal(after, before)
 
 
-# The products' tiles are 64 x 64, 128 x 128 or 256 x 128, whole, split along the contraction, or both; l >= 2 r takes up to
-# three steps together.  Tolerance: the above with the contraction K = max(m, n), whose sums' roundings grow with its root.
+# The products' tiles are 256 x 128, 128 x 128, 128 x 64 or 64 x 64, whole, split along the contraction, or both, by a count of
+# their times: these shapes take each of them.  l >= 2 r may take up to three steps together.  Tolerance: the above with the
+# contraction K = max(m, n), whose sums' roundings grow with its root.
 @pytest.mark.parametrize("shape,dtype", [
-    ((513, 3590), torch.float32), ((3590, 513), torch.bfloat16),     # 128 x 128 split 17 times
-    ((2970, 2409), torch.float32),                                   # 128 x 128
-    ((1781, 2810), torch.float32), ((1781, 2810), torch.float16),    # 256 x 128 split 4 times
-    ((3048, 3035), torch.float32), ((3048, 3035), torch.bfloat16),   # whole rounds and split tiles of each kind
-    ((449, 1941), torch.float16), ((150, 9001), torch.float32), ((9001, 130), torch.float32),
-    ((9, 269, 2656), torch.bfloat16), ((8, 1157, 416), torch.float32), ((3, 1801, 600), torch.float32)])
+    ((513, 3590), torch.float32), ((3590, 513), torch.bfloat16), ((2970, 2409), torch.float32), ((1781, 2810), torch.float32),
+    ((1781, 2810), torch.float16), ((3048, 3035), torch.float32), ((3048, 3035), torch.bfloat16), ((3712, 2152), torch.float32),
+    ((5, 2261, 1905), torch.float32), ((556, 2099), torch.float16), ((2012, 2601), torch.bfloat16), ((2012, 2601), torch.float32),
+    ((449, 1941), torch.float16), ((150, 9001), torch.float32), ((9001, 130), torch.float32), ((9, 269, 2656), torch.bfloat16),
+    ((8, 1157, 416), torch.float32), ((3, 1801, 600), torch.float32)])
 def test_larger(shape, dtype):
     from step_amd import optim
     m, n = shape[-2:]
