@@ -465,11 +465,13 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     }
 }
 
-// Tiles: 64 MT x 64 NT, a wave's share 32 MT x 32 NT.  The variants V: 0 is 256 x 128, 1 128 x 128, 2 128 x 64 and 3 64 x 64, for
-// products too small to fill the CUs with larger ones.
-constexpr int VARIANTS = 4;
-constexpr int mt_of(int v) { return v == 0 ? 4 : v == 3 ? 1 : 2; }
-constexpr int nt_of(int v) { return v < 2 ? 2 : 1; }
+// Tiles: 64 MT x 64 NT, a wave's share 32 MT x 32 NT.  The variants V: 0 is 256 x 128, 1 and 2 128 x 128, 3 128 x 64 and 4 64 x 64,
+// for products too small to fill the CUs with larger ones.  Of 2, 3 and 4 two lie in a CU, and one tile's beginning and end pass
+// beside the other's products; 1 has the CU to itself and twice the stages in flight.
+constexpr int VARIANTS = 5;
+constexpr int mt_of(int v) { return v == 0 ? 4 : v == 4 ? 1 : 2; }
+constexpr int nt_of(int v) { return v < 3 ? 2 : 1; }
+constexpr int per_cu(int v) { return v < 2 ? 1 : 2; }
 // The products of the hi parts, and the two small terms in sums of their own, so that the large sum is rounded once per product
 // and not three times.
 template <int V>
@@ -499,7 +501,7 @@ __device__ __forceinline__ void multiply(Acc<V>& acc, const Frag<V>& f) {
 
 template <int V>
 constexpr int stages_of() {
-    return V == 0 ? 3 : V == 2 ? 3 : 4;
+    return V == 0 || V == 3 ? 3 : V == 2 ? 2 : 4;
 }
 // acc += rows [i0, i0 + 64 MT) of A times rows [j0, j0 + 64 NT) of B over the stages [s0, s1): operands packed alike, K along both.
 // A stage lies in LDS as rows of 128 bytes whose eight 16-byte pieces are in the order piece ^ order(row): 16 neighbouring rows
@@ -512,7 +514,7 @@ template <int V>
 __device__ __forceinline__ void main_loop(Acc<V>& acc, const char* A, const char* B, int K, int i0, int j0, int s0, int s1, char* lds) {
     constexpr int MT = mt_of(V), NT = nt_of(V), TM = 64 * MT, TN = 64 * NT, STAGE = (TM + TN) * ROWB, NST = stages_of<V>();
     constexpr int NA = TM / 32, NB = TN / 32, NL = NA + NB;                  // a wave's copies, of 8 rows each
-    constexpr int GROUPS = V == 0 ? 12 : V == 1 ? 4 : V == 2 ? 3 : 1;        // reads are issued in so many parts, a product between two
+    constexpr int GROUPS = V == 0 ? 12 : V < 3 ? 4 : V == 3 ? 3 : 1;        // reads are issued in so many parts, a product between two
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = lane & 31, q = lane >> 5;
     const size_t pitch = (size_t)(K / KS) * ROWB;
     const int lrow = lane >> 3, piece = (lane & 7) ^ lrow, order = (l31 & 7) ^ ((l31 >> 3) & 1);
@@ -777,7 +779,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
 // Blocks [0, full): a tile each, the card's CUs filled `full / 256` times.  The tiles that are left share the card: `splits`
 // blocks a tile, each with a part of the contraction, whose sums ns_join_kernel adds up.
 template <int PROD, int V, typename T>
-__global__ __launch_bounds__(256, 1) void ns_product_kernel(const Big p, int tiles, int full, int splits) {
+__global__ __launch_bounds__(256, per_cu(V)) void ns_product_kernel(const Big p, int tiles, int full, int splits) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     // blocks go to the eight XCDs in turn: each gets neighbouring tiles, whose operands its L2 then holds
     auto neighbours = [](int b, int n) { return (b & 7) * (n >> 3) + min(b & 7, n & 7) + (b >> 3); };
@@ -862,8 +864,8 @@ Share share(int v, long long tiles, long long total) {
     return s;
 }
 double cycles(const Share& s, int stages) {
-    static const double stage[VARIANTS] = {2290, 1150, 690, 480}, end[VARIANTS] = {18000, 11000, 14000, 7000};
-    const double one = stage[s.v], ends = end[s.v], more = s.v < 2 ? 1.0 : 0.5;   // (two small tiles are in a CU at a time)
+    static const double stage[VARIANTS] = {2290, 1150, 1150, 690, 480}, end[VARIANTS] = {18000, 11000, 10000, 14000, 7000};
+    const double one = stage[s.v], ends = end[s.v], more = per_cu(s.v) == 1 ? 1.0 : 0.5;
     const int rounds = s.full / CUS;
     double c = rounds * stages * one + (rounds ? 1 + (rounds - 1) * more : 0) * ends;
     if (s.rest) c += (s.splits > 1 ? (stages + s.splits - 1) / s.splits * one + ends + 12000 + 150 * s.rest : stages * one + (rounds ? more : 1) * ends);
@@ -895,7 +897,9 @@ Layout layout_of(int nb, int r, int l) {
         Share s{};
         for (int v = 0; v < VARIANTS; ++v) {
             const int mt = mt_of(v), nt = nt_of(v), cols = step::ceil_div(r, 64 * nt);
-            const Share t = fastest(v, tri ? tri_tiles(cols, mt / nt) : (long long)step::ceil_div(l, 64 * mt) * cols, nb, stages);
+            const long long tiles = tri ? tri_tiles(cols, mt / nt) : (long long)step::ceil_div(l, 64 * mt) * cols;
+            if (v == 2 && tiles * nb <= CUS) continue;       // one tile a CU: two stages are too few
+            const Share t = fastest(v, tiles, nb, stages);
             s = v == 0 ? t : best(s, t, stages);
         }
         return s;
@@ -1011,7 +1015,8 @@ int check(const step_ns_item* items, int count) {
 template <int PROD, int V, typename T>
 int product_of(const Big& p, const Share& s, hipStream_t st) {
     auto kern = ns_product_kernel<PROD, V, T>;
-    constexpr size_t lds = stages_of<V>() * 64 * (mt_of(V) + nt_of(V)) * ROWB;
+    constexpr size_t loop = stages_of<V>() * 64 * (mt_of(V) + nt_of(V)) * ROWB, end = 64 * mt_of(V) * pitch_of<PROD, 64 * nt_of(V)>() * sizeof(float);
+    constexpr size_t lds = loop > end ? loop : end;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) {
         step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
@@ -1023,8 +1028,13 @@ int product_of(const Big& p, const Share& s, hipStream_t st) {
 }
 template <int PROD, typename T>
 int product(const Big& p, const Share& s, hipStream_t st) {
-    return s.v == 0 ? product_of<PROD, 0, T>(p, s, st) : s.v == 1 ? product_of<PROD, 1, T>(p, s, st) :
-           s.v == 2 ? product_of<PROD, 2, T>(p, s, st) : product_of<PROD, 3, T>(p, s, st);
+    switch (s.v) {
+        case 0: return product_of<PROD, 0, T>(p, s, st);
+        case 1: return product_of<PROD, 1, T>(p, s, st);
+        case 2: return product_of<PROD, 2, T>(p, s, st);
+        case 3: return product_of<PROD, 3, T>(p, s, st);
+        default: return product_of<PROD, 4, T>(p, s, st);
+    }
 }
 template <typename T>
 int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
