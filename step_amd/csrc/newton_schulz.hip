@@ -20,7 +20,7 @@
 //   contraction.  A and q(A) are symmetric: only the tiles on and over the diagonal are computed.  Bound by the matrix cores where
 //   the products fill the card (4096 x 4096: X's update 355 us, 1.16 PFLOP/s of f16 products, the cores busy in 65 % of the
 //   cycles at the 1.8 GHz that their power leaves; a plain f16 product of 8192^3 reaches 1.02), by the chain of r x r products
-//   otherwise (256 x 19200: 14 of them, 6 us each, of 176).  A value under 2^-28 of the norm keeps fewer bits: its error is 2^-39.
+//   otherwise (256 x 19200: 14 of them, 6 us each, of 170).  A value under 2^-28 of the norm keeps fewer bits: its error is 2^-39.
 #include <vector>
 #include "rows.h"
 
@@ -855,16 +855,20 @@ struct Share {
     int v, tiles, full, rest, splits;
 };
 // The variant that takes the least time by this count, in cycles at the 1.8 GHz of a full card: a stage 2290 at 256 x 128 a tile (1536
-// of them on the matrix cores), 1150 at 128 x 128, 690 at 128 x 64, 480 at 64 x 64; a tile's beginning and end, half of which two
-// small tiles in a CU share; writing the parts of split tiles and joining them.  All five steps in us, as chosen / tiles never split /
-// of 128 columns / of 256 x 128 only: 4096 x 4096 fp32 3655 / 4060 / 3657 / 3690, 256 x 19200 176 / 385 / 260 / 368, 512 x 512
-// 133 / 132 / 190 / 253, three stacked 4101 x 1030 bf16 682 / 689 / 761 / 895, 1024 x 4096 300 / 315 / 397 / 493.
+// of them on the matrix cores), 1150 and 1180 at 128 x 128, 690 at 128 x 64, 480 at 64 x 64; a tile's beginning and end, half of
+// which two tiles in a CU share; writing the parts of split tiles and joining them.  All five steps in us:
+//                             as chosen   tiles never split   one 128 x 128 a CU only   128 columns only   256 x 128 only
+//   4096 x 4096 fp32               3640                4165                      3711               3640             3730
+//   3 x 4101 x 1030 bf16            655                 678                       680                762              893
+//   256 x 19200 fp32                170                 377                       177                258              371
+//   1024 x 4096 fp32                302                 315                       303                402              502
+//   512 x 512 fp32                  133                 132                       132                194              249
 Share share(int v, long long tiles, long long total) {
     Share s{v, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
     return s;
 }
 double cycles(const Share& s, int stages) {
-    static const double stage[VARIANTS] = {2290, 1150, 1150, 690, 480}, end[VARIANTS] = {18000, 11000, 10000, 14000, 7000};
+    static const double stage[VARIANTS] = {2290, 1150, 1180, 690, 480}, end[VARIANTS] = {18000, 11000, 10000, 14000, 7000};
     const double one = stage[s.v], ends = end[s.v], more = per_cu(s.v) == 1 ? 1.0 : 0.5;
     const int rounds = s.full / CUS;
     double c = rounds * stages * one + (rounds ? 1 + (rounds - 1) * more : 0) * ends;
@@ -931,7 +935,7 @@ Layout layout(int batch, int m, int n) {
     o.xt2 = take(sub * R * L * 4);
     // Steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
     // products of r x r matrices, of which each further step takes three more: where the two passes over X cost more than those
-    // (256 x 19200: 176 us, 231 step by step; 3 x 4101 x 1030 682 and 956; 400 x 900, taken step by step, 141, and 150 together).
+    // (256 x 19200: 170 us, 224 step by step; 3 x 4101 x 1030 655 and 933; 400 x 900, taken step by step, 140, and 150 together).
     // An error of A grows by a^2 = 12 in each step of a group for the smallest eigenvalues: three fp32-accurate steps cost them
     // 2e-5 of the largest, less than what X X^T over a length of 2 r is off by.
     const double passes = cycles(o.xxt, step::ceil_div(l, KS)) + cycles(o.update, step::ceil_div(r, KS));
