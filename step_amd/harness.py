@@ -155,7 +155,10 @@ class EpochRunner:
 
     def _logits(self, model, data):
         output, _ = model(data.float())
-        return torch.log(output) if getattr(model, "RETURNS_SOFTMAX", False) else output
+        if not getattr(model, "RETURNS_SOFTMAX", False):
+            return output
+        # (a probability that went down to zero would have a gradient of inf times zero)
+        return torch.log(output.clamp_min(torch.finfo(output.dtype).tiny))
 
     def per_policy(self, reward, reference=None, clip=0.2, beta=0.04, inner=2):
         """One epoch of fine-tuning on rewards: for every batch an emotion is drawn per gait from the model, rated by

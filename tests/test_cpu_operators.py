@@ -182,3 +182,19 @@ def test_sizes_beyond_the_library_are_refused():
                 "step_policy_loss": [PTR, PTR, PTR, PTR, None, None, 0.2, 0.2, 0.0, None, 0, PTR, PTR, PTR, PTR, 4, 8, 0, PTR, 1 << 20, None]}[name]
         args[at] = (1 << 31) - 1
         assert code(name, *args)[0] == -1
+
+
+def test_policy_logits_of_a_saturated_softmax():
+    """a model that answers with probabilities, one of them gone to zero: finite logits, finite gradients"""
+    from step_amd.harness import EpochRunner
+
+    class Sure:
+        RETURNS_SOFTMAX = True
+
+        def __call__(self, x):
+            return torch.softmax(x, 1), None
+    x = torch.tensor([[0.0, -200.0, 1.0]], requires_grad=True)
+    logits = EpochRunner._logits(None, Sure(), x)
+    (logits * torch.tensor([[1.0, -1.0, 0.5]])).sum().backward()
+    assert bool(logits.isfinite().all()) and bool(x.grad.isfinite().all())
+    assert torch.equal(logits[0, 0], torch.log(torch.softmax(x, 1))[0, 0])
