@@ -435,20 +435,25 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     __shared__ float sm[64][65];
     __shared__ double red[4];
     const int tid = threadIdx.x, z = blockIdx.z;
+    const Io io = shifted(p.io, (size_t)p.m * p.n * z, sizeof(T));
+    const bool tall = p.m > p.n;
+    const int i0 = blockIdx.y * 64, k0 = blockIdx.x * 64;                    // rows of the short side, columns of the long
+    float in[16];                                            // on their way while the norm is added up
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int a = 4 * j + (tid >> 6), b = tid & 63, i = i0 + (tall ? b : a), k = k0 + (tall ? a : b);
+        in[j] = i < p.r && k < p.l ? read_u<T>(io, tall ? (size_t)k * p.n + i : (size_t)i * p.n + k, false) : 0.f;
+    }
     double s = 0.0;
     for (int i = tid; i < NORM_BLOCKS; i += 256) s += p.part[(size_t)z * NORM_BLOCKS + i];
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
     const float scale = (float)((double)SX / (sqrt(red[0] + red[1] + red[2] + red[3]) + (double)p.eps));
-    const Io io = shifted(p.io, (size_t)p.m * p.n * z, sizeof(T));
-    const bool tall = p.m > p.n;
-    const int i0 = blockIdx.y * 64, k0 = blockIdx.x * 64;                    // rows of the short side, columns of the long
-    for (int e = tid; e < 4096; e += 256) {
-        const int a = e >> 6, b = e & 63;
-        const int i = i0 + (tall ? b : a), k = k0 + (tall ? a : b);
-        const float v = i < p.r && k < p.l ? read_u<T>(io, tall ? (size_t)k * p.n + i : (size_t)i * p.n + k, false) * scale : 0.f;
-        sm[i - i0][k - k0] = v;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int a = 4 * j + (tid >> 6), b = tid & 63;
+        sm[tall ? b : a][tall ? a : b] = in[j] * scale;
     }
     __syncthreads();
     char* x = p.x + (size_t)z * p.RA * p.L * 4;

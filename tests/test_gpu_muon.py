@@ -300,7 +300,7 @@ def test_inference_caches_see_a_step():
     ((1781, 2810), torch.float16), ((3048, 3035), torch.float32), ((3048, 3035), torch.bfloat16), ((3712, 2152), torch.float32),
     ((5, 2261, 1905), torch.float32), ((556, 2099), torch.float16), ((2012, 2601), torch.bfloat16), ((2012, 2601), torch.float32),
     ((449, 1941), torch.float16), ((150, 9001), torch.float32), ((9001, 130), torch.float32), ((9, 269, 2656), torch.bfloat16),
-    ((8, 1157, 416), torch.float32), ((3, 1801, 600), torch.float32)])
+    ((8, 1157, 416), torch.float32), ((3, 1801, 600), torch.float32), ((1030, 65, 70), torch.float32)])   # (1024 at a time)
 def test_larger(shape, dtype):
     from step_amd import optim
     m, n = shape[-2:]
