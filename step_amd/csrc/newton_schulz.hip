@@ -941,11 +941,10 @@ Layout layout(int batch, int m, int n) {
     o.xt2 = take(sub * R * L * 4);
     // Steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
     // products of r x r matrices, of which each further step takes three more: where the two passes over X cost more than those
-    // (256 x 19200: 170 us, 224 step by step; 3 x 4101 x 1030 655 and 933; 400 x 900, taken step by step, 140, and 150 together).
-    // An error of A grows by a^2 = 12 in each step of a group for the smallest eigenvalues: three fp32-accurate steps cost them
-    // 2e-5 of the largest, less than what X X^T over a length of 2 r is off by.
+    // (256 x 19200: 170 us, 224 step by step; 3 x 4101 x 1030 655 and 933; 400 x 900, taken step by step, 140, and 150 together; 3.8 passes' worth is
+    // where they are even: 1690 x 71 103 both ways, 2500 x 1000 311 and 277 together).
     const double passes = cycles(o.xxt, step::ceil_div(l, KS)) + cycles(o.update, step::ceil_div(r, KS));
-    o.group = l >= 2 * r && passes > 3 * cycles(o.sym, step::ceil_div(r, KS)) ? 3 : 1;
+    o.group = l >= 2 * r && passes > 3.8 * cycles(o.sym, step::ceil_div(r, KS)) ? 3 : 1;
     for (int i = 0; i < (o.group > 1 ? 4 : 2); ++i) o.r[i] = take(sub * RA * R * 4);
     // shares of split tiles: fewer than one a CU, of 256 x 128 at most.  A last part of the batch that is smaller is shared out anew.
     const bool any = sub < batch || o.xxt.splits > 1 || o.sym.splits > 1 || o.update.splits > 1;
@@ -1046,6 +1045,14 @@ int product(const Big& p, const Share& s, hipStream_t st) {
         default: return product_of<PROD, 4, T>(p, s, st);
     }
 }
+// An error of A grows by a^2 = 12 in each step of a group for the smallest eigenvalues.  fp32 results off by, together / step by step
+// (fp32 products of the library: the last figure): 10000 x 100 2.5e-6 / 0.7e-6 (1.5e-6), 6000 x 130 2.0e-6 / 0.8e-6 (1.3e-6),
+// 7000 x 160 1.8e-6 / 1.2e-6 (1.6e-6), 256 x 19200 1.5e-6 / 1.2e-6 (4.4e-6), 6000 x 1000 2.3e-6 / 1.6e-6 (2.8e-6): the narrow ones are
+// taken step by step.  Results of 16 bits are rounded far above that.
+template <typename T>
+bool together(int r) {
+    return sizeof(T) < 4 || r >= 160;
+}
 template <typename T>
 int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
     const Layout all = layout(it.batch, it.m, it.n);
@@ -1061,6 +1068,7 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
     p.part = (double*)(base + all.part);
     p.slab = (float*)(base + all.slab);
     p.x = base + all.x;
+    const int group = together<T>(p.r) ? all.group : 1;
     char* r[4];
     for (int i = 0; i < 4; ++i) r[i] = base + all.r[i];
     for (int b0 = 0; b0 < it.batch; b0 += all.sub) {
@@ -1092,7 +1100,7 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
             if (rc == STEP_OK) rc = product<POLY, float>(p, o.sym, st);
         };
         for (int s = 0; s < steps && rc == STEP_OK;) {
-            const int g = steps - s < all.group ? steps - s : all.group;
+            const int g = steps - s < group ? steps - s : group;
             char *A = r[0], *P = r[1], *Q = r[1], *W = r[2], *F = r[3];      // F: free
             p.s3 = A;
             p.scale = SA / (SX * SX);
