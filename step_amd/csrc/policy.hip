@@ -45,6 +45,11 @@ struct Args {
 struct Soft {
     float m, s;
 };
+// the same of many threads: what the rounding of one addition costs them all is not averaged out, so it takes fp64
+struct Row {
+    float m;
+    double s;
+};
 __device__ __forceinline__ float exp_of(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * L2E); }
 // for the sum, whose logarithm the loss hangs on: the product with log2 e to 48 bits, rounded once (fp32's log2 e alone is off by
 // 1.3e-8, the same way for all elements: log probabilities 3.5e-8 too low on average over 613 classes)
@@ -54,40 +59,67 @@ __device__ __forceinline__ float exp_for_sum(float x, float m) {
 }
 __device__ __forceinline__ float finite_or_0(float m) { return m == -__builtin_inff() ? 0.f : m; }   // no -inf - -inf
 
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    const u32x2 q = __builtin_bit_cast(u32x2, v);
+    u32x2 r;
+    r[0] = (unsigned)__builtin_amdgcn_mov_dpp((int)q[0], CTRL, 0xf, 0xf, true);
+    r[1] = (unsigned)__builtin_amdgcn_mov_dpp((int)q[1], CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+    const u32x2 q = __builtin_bit_cast(u32x2, v);
+    u32x2 r;
+    r[0] = (unsigned)__builtin_amdgcn_readlane((int)q[0], lane);
+    r[1] = (unsigned)__builtin_amdgcn_readlane((int)q[1], lane);
+    return __builtin_bit_cast(double, r);
+}
 template <int G>
-__device__ __forceinline__ Soft join(const Soft w, Soft* sm) {
-    if constexpr (G <= 64) {
-        return w;
-    } else {
+__device__ __forceinline__ double wave_sum64(double v) {       // (wave_reduce's steps)
+    v += dpp64<0xb1>(v);
+    v += dpp64<0x4e>(v);
+    v += dpp64<0x141>(v);
+    if constexpr (G >= 16) v += dpp64<0x140>(v);
+    if constexpr (G >= 64) v = (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+    return v;
+}
+// over the G threads that have the maximum and sum of their elements, the same bits in all of them
+template <int G>
+__device__ __forceinline__ Row reduce(float m, double s, Row* sm) {
+    constexpr int W = G < 64 ? G : 64;
+    Row w;
+    w.m = wave_reduce<W>(m, [](float a, float b) { return fmaxf(a, b); });
+    w.s = wave_sum64<W>(s * exp_for_sum(m, finite_or_0(w.m)));
+    if constexpr (G > 64) {
         if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = w;
         __syncthreads();
-        Soft r = sm[0];
+        w = sm[0];
 #pragma unroll
-        for (int i = 1; i < G / 64; ++i) r.m = fmaxf(r.m, sm[i].m);
-        const float m0 = finite_or_0(r.m);
-        r.s = 0.f;
+        for (int i = 1; i < G / 64; ++i) w.m = fmaxf(w.m, sm[i].m);
+        const float m0 = finite_or_0(w.m);
+        w.s = 0.0;
 #pragma unroll
-        for (int i = 0; i < G / 64; ++i) r.s += sm[i].s * exp_for_sum(sm[i].m, m0);
-        return r;
+        for (int i = 0; i < G / 64; ++i) w.s += sm[i].s * exp_for_sum(sm[i].m, m0);
     }
+    return w;
 }
 
 // exp and log2 in fp64 for a row's scalars, from their series: a third of the registers and of the time that the general
 // functions take, which one thread of a block spends while the others wait.
 // log2 s = e + log2 m, s = m 2^e with m in [sqrt 1/2, sqrt 2): log m = 2 atanh t, t = (m - 1) / (m + 1), |t| <= 0.172, to t^13:
 // the rest is under 2 t^15 / 15 = 5e-13.  (s is 1 or more, or NaN, or comes from a row that allows nothing, where m is -inf.)
-__device__ __forceinline__ double log2_of(float s) {
-    int e = __builtin_amdgcn_frexp_expf(s);
-    float m = __builtin_amdgcn_frexp_mantf(s);
-    if (m < 0.70710678f) {
-        m *= 2.f;
+__device__ __forceinline__ double log2_of(double s) {
+    int e = __builtin_amdgcn_frexp_exp(s);
+    double m = __builtin_amdgcn_frexp_mant(s);
+    if (m < 0.70710678) {
+        m *= 2.0;
         --e;
     }
-    const double d = (double)m + 1.0;
+    const double d = m + 1.0;
     double r = __builtin_amdgcn_rcp(d);
     r = r * (2.0 - d * r);
     r = r * (2.0 - d * r);
-    const double t = ((double)m - 1.0) * r, u = t * t;
+    const double t = (m - 1.0) * r, u = t * t;
     const double a = 1.0 + u * (1.0 / 3 + u * (1.0 / 5 + u * (1.0 / 7 + u * (1.0 / 9 + u * (1.0 / 11 + u * (1.0 / 13))))));
     return (double)e + (2.0 / LN2) * (t * a);
 }
@@ -112,7 +144,7 @@ __device__ __forceinline__ double exp_of64(double x) {
 }
 
 // the row's scalars: returns dL/dlp / count (times the upstream gradient), adds the row to the block's sums
-__device__ __forceinline__ float row_scalars(const Args& p, long long row, Soft f, float za, bool valid, double count,
+__device__ __forceinline__ float row_scalars(const Args& p, long long row, const Row& f, float za, bool valid, double count,
                                              double* sums, bool write = true) {
     const double lp = valid ? (double)za - (double)f.m - log2_of(f.s) * LN2 : (double)__builtin_nanf("");
     const double a = p.adv[row], ratio = exp_of64(lp - (double)p.old_logp[row]);
@@ -202,20 +234,11 @@ __device__ __forceinline__ void add_packs(Soft& f, Pack<T, N>* v) {
         for (int k = 0; k < U; ++k) forget(v[i + k]);
     }
 }
-// over the G threads that have the maximum and sum of their elements, the same bits in all of them
-template <int G>
-__device__ __forceinline__ Soft reduce(Soft f, Soft* sm) {
-    const float m = wave_reduce<G < 64 ? G : 64>(f.m, [](float a, float b) { return fmaxf(a, b); });
-    f.s = wave_reduce<G < 64 ? G : 64>(f.s * exp_for_sum(f.m, finite_or_0(m)), [](float a, float b) { return a + b; });
-    f.m = m;
-    return join<G>(f, sm);
-}
-
 // G threads a row, NV packs of N elements a thread (the last LAST of them may not fit)
 template <typename T, int N, int NV, int LAST, int G>
 __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_kernel(const Args p) {
     constexpr int BLOCK = G < 256 ? 256 : G, RPB = BLOCK / G;
-    __shared__ Soft sm[2][G > 64 ? G / 64 : 1];
+    __shared__ Row sm[2][G > 64 ? G / 64 : 1];
     __shared__ float coef_s;
     if (p.upstream && p.skip_one && *p.upstream == 1.f) return;
     const int lane = threadIdx.x % G;
@@ -247,25 +270,25 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
         const float za = lane == 0 && valid ? (float)z[action] : 0.f;
         own.fill(v, (T)-__builtin_inff());
         add_packs<T, N, NV>(f, v);
-        f = reduce<G>(f, sm[turn]);
+        const Row w = reduce<G>(f.m, (double)f.s, sm[turn]);
         turn ^= 1;
         float coef;
         if constexpr (G <= 64) {
             double add[3] = {0.0, 0.0, 0.0};
-            coef = row_scalars(p, row, f, __shfl(za, (threadIdx.x & 63) & ~(G - 1), 64), valid, count, add);
+            coef = row_scalars(p, row, w, __shfl(za, (threadIdx.x & 63) & ~(G - 1), 64), valid, count, add);
             if (lane == 0)
                 for (int k = 0; k < 3; ++k) sums[k] += add[k];
         } else {
-            if (threadIdx.x == 0) coef_s = row_scalars(p, row, f, za, valid, count, sums);
+            if (threadIdx.x == 0) coef_s = row_scalars(p, row, w, za, valid, count, sums);
             __syncthreads();
             coef = coef_s;
         }
         if (!g) continue;
-        const float scale = -coef / f.s;
+        const float scale = -coef / (float)w.s;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) own.store(g, i, gradient_of<T, N>(v[i], f.m, scale));
+        for (int i = 0; i < NV; ++i) own.store(g, i, gradient_of<T, N>(v[i], w.m, scale));
         // the thread that wrote the action's element writes it once more
-        if (valid && lane == action / N % G) g[action] = (T)(exp_of((float)z[action], f.m) * scale + coef);
+        if (valid && lane == action / N % G) g[action] = (T)(exp_of((float)z[action], w.m) * scale + coef);
     }
     if (!p.upstream) block_sums<BLOCK>(p.part, sums);
 }
@@ -276,8 +299,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
 // 2000 x 100000 fp32: 465 us, 5.2 TB/s of what it reads and writes; 4 or 16 packs: within 4 % either way).
 constexpr int PART_PACKS = 8;
 template <typename T, int N, bool GRAD>
-__global__ __launch_bounds__(256) void policy_parts_kernel(const Args p, Soft* soft, int parts, int span) {
-    __shared__ Soft sm[2][4];
+__global__ __launch_bounds__(256) void policy_parts_kernel(const Args p, Row* soft, int parts, int span) {
+    __shared__ Row sm[2][4];
     __shared__ float coef_s[2];
     if (p.upstream && p.skip_one && *p.upstream == 1.f) return;
     const int tid = threadIdx.x;
@@ -304,24 +327,25 @@ __global__ __launch_bounds__(256) void policy_parts_kernel(const Args p, Soft* s
         }
         Pack<T, N> v[PART_PACKS];
         if (!GRAD || g) own.load(v, z + c0);                 // (a pack at the end of a short last part lies in the part before)
-        Soft f{-__builtin_inff(), 0.f};
         if constexpr (!GRAD) {
+            Soft t{-__builtin_inff(), 0.f};
             own.fill(v, (T)-__builtin_inff());
-            add_packs<T, N, PART_PACKS>(f, v);
-            f = reduce<256>(f, sm[turn]);
+            add_packs<T, N, PART_PACKS>(t, v);
+            const Row f = reduce<256>(t.m, (double)t.s, sm[turn]);
             turn ^= 1;
             if (tid == 0) soft[item] = f;
         } else {
             const long long a64 = p.actions[row];
             const bool valid = a64 >= 0 && a64 < p.classes;
             const float za = tid == 0 && valid ? (float)z[a64] : 0.f;
+            Row f{-__builtin_inff(), 0.0};
             for (int i = tid; i < parts; i += 256) {
-                const Soft o = soft[row * parts + i];
+                const Row o = soft[row * parts + i];
                 const float m = fmaxf(f.m, o.m), m0 = finite_or_0(m);
                 f.s = f.s * exp_for_sum(f.m, m0) + o.s * exp_for_sum(o.m, m0);
                 f.m = m;
             }
-            f = reduce<256>(f, sm[turn]);
+            f = reduce<256>(f.m, f.s, sm[turn]);
             if (tid == 0) {
                 double add[3] = {0.0, 0.0, 0.0};
                 coef_s[turn] = row_scalars(p, row, f, za, valid, count, add, part == 0);
@@ -332,7 +356,7 @@ __global__ __launch_bounds__(256) void policy_parts_kernel(const Args p, Soft* s
             const float coef = coef_s[turn];
             turn ^= 1;
             if (!g) continue;
-            const float scale = -coef / f.s;
+            const float scale = -coef / (float)f.s;
 #pragma unroll
             for (int i = 0; i < PART_PACKS; ++i) own.store(g + c0, i, gradient_of<T, N>(v[i], f.m, scale));
             // the thread that wrote the action's element writes it once more
@@ -435,7 +459,7 @@ void launch(const Plan& pl, int blocks, const Args& a, hipStream_t st) {
     else launch_nv<T, N, 1024, 10, 16>(pl.nv, blocks, a, st);
 }
 template <typename T>
-void launch_parts(int parts, int span, int blocks, const Args& a, Soft* soft, hipStream_t st) {
+void launch_parts(int parts, int span, int blocks, const Args& a, Row* soft, hipStream_t st) {
     constexpr int N = 16 / (int)sizeof(T);
     if (!a.upstream) hipLaunchKernelGGL((policy_parts_kernel<T, N, false>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
     hipLaunchKernelGGL((policy_parts_kernel<T, N, true>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
@@ -446,7 +470,7 @@ void launch_parts(int parts, int span, int blocks, const Args& a, Soft* soft, hi
 extern "C" size_t step_policy_loss_ws_bytes(long long rows, int classes) {
     if (rows <= 0 || classes <= 0 || classes > 1 << 30) return 0;
     int span;                                                // (fp32's parts: a 16-bit type has fewer)
-    const size_t soft = plan(classes, STEP_F32).g ? 0 : (size_t)rows * parts_of(classes, 4, span) * sizeof(Soft);
+    const size_t soft = plan(classes, STEP_F32).g ? 0 : (size_t)rows * parts_of(classes, 4, span) * sizeof(Row);
     return (1 + 3 * (size_t)MAX_BLOCKS) * sizeof(double) + soft;
 }
 
@@ -481,7 +505,7 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
     auto go = [&](auto t) {
         using T = decltype(t);
         if (pl.g) launch<T>(pl, blocks, a, st);
-        else launch_parts<T>(parts, span, blocks, a, (Soft*)(part + 3 * MAX_BLOCKS), st);
+        else launch_parts<T>(parts, span, blocks, a, (Row*)(part + 3 * MAX_BLOCKS), st);
     };
     if (dtype == STEP_F32) go(float());
     else if (dtype == STEP_BF16) go(bf16());
