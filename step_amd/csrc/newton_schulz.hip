@@ -20,7 +20,9 @@
 //   contraction.  A and q(A) are symmetric: only the tiles on and over the diagonal are computed.  Bound by the matrix cores where
 //   the products fill the card (4096 x 4096: X's update 355 us, 1.16 PFLOP/s of f16 products, the cores busy in 65 % of the
 //   cycles at the 1.8 GHz that their power leaves; a plain f16 product of 8192^3 reaches 1.02), by the chain of r x r products
-//   otherwise (256 x 19200: 14 of them, 6 us each, of 170).  A value under 2^-28 of the norm keeps fewer bits: its error is 2^-39.
+//   otherwise (256 x 19200: 14 of them, 6 us each, of 170).  An element's error is 2^-23 of it, or 2^-39 where it is under 2^-17
+//   (f16's subnormals hold its lo): of the matrix's size, since X is lifted by a power of two as long as |G| is far below eps
+//   and X with it (lift() below).
 #include <vector>
 #include "rows.h"
 
@@ -364,18 +366,28 @@ constexpr int ROWB = 128;                         // bytes of a row's stage: 32 
 constexpr float SX = 16384.f, SA = 16384.f, SQ[3] = {8192.f, 4096.f, 1024.f};
 constexpr int CUS = 256;
 constexpr int NORM_BLOCKS = 1024;
+constexpr int BATCH = 1024;                       // matrices of a stack at a time, at most
 
 struct Big {
     Io io;
     int m, n, r, l, R, L, RA;                     // R, L: r and l rounded up to whole tiles; RA: rows that X and A have
     float eps;
-    double* part;                                 // [batch][NORM_BLOCKS] sums of squares
+    double* part;                                 // [batch][NORM_BLOCKS] sums of squares, and before them [BATCH] -log2 |X_0| in floats
     char *x, *xt, *xt2;                           // packed matrices, one after the other for the batch
     const char *s1, *s2;                          // R x R (RA rows) operands of a product, and its result
     char* s3;
     float scale;                                  // result's scale over the operands'
+    int from : 16, by : 16;                       // the step whose lift a product's operands have, and how many steps further its result is
     float* slab;                                  // shares of split tiles
 };
+
+// |X_k| <= q(0)^k |X_0|, and |X_0| = |G| / (|G| + eps) may be anything below 1: X_k is held times 2^lift(k), the largest power with
+// which that bound stays at 1 or below (0 once the bound reaches 1/2, as from the start where |G| is over eps), A_k times its square.
+__device__ __forceinline__ float* heads(const Big& p) { return (float*)p.part - BATCH; }
+__device__ __forceinline__ int lift(float head, int k) {
+    constexpr float GROWTH = 1.78429458f;         // log2 QA
+    return (int)fmaxf(floorf(head - (float)k * GROWTH), 0.f);
+}
 
 // sums of squares in fp64; with the momentum's update in the optimizer's form (4096 x 4096 fp32: 17 us, 4.0 TB/s, once per call)
 template <typename T>
@@ -450,11 +462,18 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
     if ((tid & 63) == 0) red[tid >> 6] = s;
     __syncthreads();
-    const float scale = (float)((double)SX / (sqrt(red[0] + red[1] + red[2] + red[3]) + (double)p.eps));
+    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]), over = norm + (double)p.eps, size = norm / over;
+    // (head: 0 of 0 / 0, and where there are NaN or infinities)
+    const float head = size > 0.0 ? -((float)__builtin_amdgcn_frexp_exp(size) + __builtin_amdgcn_logf((float)__builtin_amdgcn_frexp_mant(size))) : 0.f;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) heads(p)[z] = head;
+    // 2^lift SX / (norm + eps) in two factors, for either may be beyond fp32
+    const double scale = (double)SX / over;
+    const int power = __builtin_amdgcn_frexp_exp(scale) + lift(head, 0);
+    const float factor = (float)__builtin_amdgcn_frexp_mant(scale);
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const int a = 4 * j + (tid >> 6), b = tid & 63;
-        sm[tall ? b : a][tall ? a : b] = in[j] * scale;
+        sm[tall ? b : a][tall ? a : b] = __builtin_ldexpf(in[j], power) * factor;
     }
     __syncthreads();
     char* x = p.x + (size_t)z * p.RA * p.L * 4;
@@ -699,7 +718,7 @@ __device__ __forceinline__ void transposed(const float* sm, F to) {
 }
 
 template <int PROD, int ROWS, int TN, typename T>
-__device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, int j0) {
+__device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, int j0, float head) {
     constexpr int EP = pitch_of<PROD, TN>(), STEP = 256 / (TN / 8);           // rows that the threads' packs of eight neighbours cover
     constexpr int N = ROWS < STEP ? 1 : ROWS / STEP, M = N < 8 ? N : 8;      // N times, M of them at a time
     const int row = threadIdx.x / (TN / 8), col = threadIdx.x % (TN / 8) * 8;
@@ -707,6 +726,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
         char* to = p.s3 + (size_t)z * p.RA * p.R * 4;
         const char* a = p.s1 + (size_t)z * p.RA * p.R * 4;
         const int cb = j0 / TN;
+        const float qb = PROD == POLY ? __builtin_ldexpf((float)QB * (SQ[0] / SA), -2 * lift(head, p.from)) : 0.f;
         for (int u = 0; u < N; u += M) {
             f16x8 hi[M], lo[M];
             if constexpr (PROD == POLY) {
@@ -728,7 +748,7 @@ __device__ __forceinline__ void finish(const Big& p, float* sm, int z, int i0, i
                 for (int e = 0; e < 8; ++e) {
                     v[e] = sm[i * EP + col + e];
                     if constexpr (PROD == POLY) {
-                        v[e] += (float)QB * (SQ[0] / SA) * ((float)hi[k][e] + (float)lo[k][e]);
+                        v[e] += qb * ((float)hi[k][e] + (float)lo[k][e]);
                         if (i0 + i == j0 + col + e) v[e] += (float)QA * SQ[0];
                         sm[i * EP + col + e] = v[e];
                     }
@@ -799,6 +819,7 @@ __global__ __launch_bounds__(256, per_cu(V)) void ns_product_kernel(const Big p,
     const bool whole = (int)blockIdx.x < full || splits == 1;
     int z, i0, j0;
     locate<PROD, V>(p, tile, z, i0, j0, tiles);
+    const float head = PROD == XXT ? 0.f : heads(p)[z];      // (read here, it has come before it is looked at)
     const char *A, *B;
     int K;
     if constexpr (PROD == XXT) {
@@ -824,15 +845,21 @@ __global__ __launch_bounds__(256, per_cu(V)) void ns_product_kernel(const Big p,
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc.v[a][b][e] = acc.w[a][b][e] = 0.f;
     main_loop(acc, A, B, K, i0, j0, s0, s1, smem);
-    const float f = p.scale;
+    // the operands' lift off, the result's on (the last result's power is not one with the factor: it may be beyond fp32)
+    int power = 0;
+    if constexpr (PROD == POLY) power = -4 * lift(head, p.from);
+    else if constexpr (PROD == SYM || PROD == UPDATE) power = (PROD == SYM ? 2 : 1) * (lift(head, p.from + p.by) - lift(head, p.from));
+    else if constexpr (PROD == RESULT) power = -lift(head, p.from);
+    const float f = PROD == RESULT ? p.scale : __builtin_ldexpf(p.scale, power);
+    auto scaled = [=](float v) { return PROD == RESULT ? __builtin_ldexpf(v * f, power) : v * f; };
     if (whole) {
         float* sm = (float*)smem;
-        each(acc, [&](int i, int j, float v) { sm[i * pitch_of<PROD, TN>() + j] = v * f; });
+        each(acc, [&](int i, int j, float v) { sm[i * pitch_of<PROD, TN>() + j] = scaled(v); });
         __syncthreads();
-        finish<PROD, 64 * MT, TN, T>(p, sm, z, i0, j0);
+        finish<PROD, 64 * MT, TN, T>(p, sm, z, i0, j0, head);
     } else {
         float* slab = p.slab + ((size_t)(tile - full) * splits + split) * (64 * MT * TN);
-        each(acc, [&](int i, int j, float v) { slab[i * TN + j] = v * f; });
+        each(acc, [&](int i, int j, float v) { slab[i * TN + j] = scaled(v); });
     }
 }
 // eight rows of a split tile, its shares added in order (16 tiles of 16 shares: 6 us)
@@ -842,6 +869,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, in
     __shared__ __attribute__((aligned(16))) float sm[8 * EP];
     int z, i0, j0;
     locate<PROD, V>(p, full + blockIdx.x, z, i0, j0, tiles);
+    const float head = PROD == POLY ? heads(p)[z] : 0.f;
     const int i = threadIdx.x / (TN / 4), j = threadIdx.x % (TN / 4) * 4;
     if (i < 8) {
         const float* slab = p.slab + (size_t)blockIdx.x * splits * (64 * MT * TN) + (blockIdx.y * 8 + i) * TN + j;
@@ -852,7 +880,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(const Big p, int tiles, in
         for (int e = 0; e < 4; ++e) sm[i * EP + j + e] = v[e];
     }
     __syncthreads();
-    finish<PROD, 8, TN, T>(p, sm, z, i0 + blockIdx.y * 8, j0);
+    finish<PROD, 8, TN, T>(p, sm, z, i0 + blockIdx.y * 8, j0, head);
 }
 
 // ---------------------------------------------------------------------------------------------- host
@@ -925,7 +953,7 @@ Layout layout(int batch, int m, int n) {
     const size_t most = (size_t)1 << 28;                           // elements of X at a time
     const size_t fit = most / ((size_t)step::round_up(r, 256) * step::round_up(l, 256));
     int sub = (int)(fit < (size_t)batch ? fit : (size_t)batch);
-    sub = sub < 1 ? 1 : sub > 1024 ? 1024 : sub;
+    sub = sub < 1 ? 1 : sub > BATCH ? BATCH : sub;
     Layout o = layout_of(sub, r, l);
     o.sub = sub;
     size_t at = 0;
@@ -935,7 +963,7 @@ Layout layout(int batch, int m, int n) {
         return here;
     };
     const size_t R = o.R, L = o.L, RA = o.RA;
-    o.part = take((size_t)sub * NORM_BLOCKS * sizeof(double));
+    o.part = take(BATCH * sizeof(float) + (size_t)sub * NORM_BLOCKS * sizeof(double)) + BATCH * sizeof(float);
     o.x = take(sub * RA * L * 4);
     o.xt = take(sub * R * L * 4);
     o.xt2 = take(sub * R * L * 4);
@@ -1085,15 +1113,18 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
         hipLaunchKernelGGL(ns_norm_kernel<T>, dim3(NORM_BLOCKS, nb), dim3(256), 0, st, p);
         hipLaunchKernelGGL(ns_pack_kernel<T>, dim3(p.L / 64, p.R / 64, nb), dim3(256), 0, st, p);
         int rc = STEP_OK;
-        // s3 <- s1 s2, scales f1, f2 -> f3
-        auto sym = [&](const char* s1, float f1, const char* s2, float f2, char* s3, float f3) {
+        // s3 <- s1 s2, scales f1, f2 -> f3; from A_k to A_k + 1 where it is that
+        auto sym = [&](const char* s1, float f1, const char* s2, float f2, char* s3, float f3, int k = -1) {
+            p.from = k;
+            p.by = k < 0 ? 0 : 1;
             p.s1 = s1;
             p.s2 = s2;
             p.s3 = s3;
             p.scale = f3 / (f1 * f2);
             if (rc == STEP_OK) rc = product<SYM, float>(p, o.sym, st);
         };
-        auto poly = [&](const char* a, char* to) {
+        auto poly = [&](const char* a, char* to, int k) {
+            p.from = k;
             p.s1 = a;
             p.s3 = to;
             p.scale = (float)QC * SQ[0] / (SA * SA);
@@ -1105,14 +1136,14 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
             p.s3 = A;
             p.scale = SA / (SX * SX);
             rc = product<XXT, float>(p, o.xxt, st);
-            poly(A, Q);
+            poly(A, Q, s);
             for (int k = 1; k < g; ++k) {
                 sym(Q, SQ[0], A, SA, W, SA);                                 // A <- q(A) A q(A)
-                sym(W, SA, Q, SQ[0], A, SA);
+                sym(W, SA, Q, SQ[0], A, SA, s + k - 1);
                 if (k > 1) {                                                 // (the last q(A) is no longer needed, P is)
                     F = Q;
                 }
-                poly(A, F);
+                poly(A, F, s + k);
                 Q = F;
                 sym(Q, SQ[0], P, SQ[k - 1], W, SQ[k]);
                 F = P;
@@ -1120,6 +1151,8 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
                 W = F;
             }
             p.s2 = P;
+            p.from = s;
+            p.by = g;
             s += g;
             p.scale = s < steps ? SX / (SQ[g - 1] * SX) : 1.f / (SQ[g - 1] * SX);
             if (rc == STEP_OK) rc = s < steps ? product<UPDATE, float>(p, o.update, st) : product<RESULT, T>(p, o.update, st);

@@ -363,3 +363,42 @@ def orthogonalised32(g):
         s = x @ x.mT.contiguous()
         x = A * x + (B * s + C * (s @ s)) @ x
     return x.mT if tall else x
+
+
+# What a size below eps may cost.  X_0 = g / (|g| + eps) is small by any power there, and so are the first steps' results, which grow
+# by a = 3.4445 each: the tolerance is relative and the same as for any other size, since nothing in the formula is less exact there.
+# References: the result's type rounds them where it has no such small numbers (half a unit of its smallest one, 2^-150 in fp32).
+@pytest.mark.parametrize("m,n", [(30, 90), (120, 100), (300, 1300), (9001, 170), (2000, 600)])
+def test_sizes_far_below_eps(m, n):
+    from step_amd import optim
+    g = matrices(m, n, seed=3)
+    g = g / g.norm()
+    for e in (-7, -9, -11, -12, -13, -15, -18, -25, -34):
+        for steps in (1, 5, 7):
+            t = g * 10.0 ** e
+            close(optim.newton_schulz(t, steps=steps), orthogonalised(t, steps), tolerance(m, n, torch.float32) * (1 if steps < 6 else 5), (e, steps))
+    for eps in (1e-3, 1.0, 1e20, 1e-30):
+        for e in (-3, -8, -30):
+            t = g * 10.0 ** e
+            ref = orthogonalised(t, 5, float(torch.tensor(eps)))
+            if float(ref.norm()) > 1e-30:
+                close(optim.newton_schulz(t, eps=eps), ref, tolerance(m, n, torch.float32), (e, eps))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_stack_of_sizes(dtype):
+    """each matrix of a stack has its own size: one among ordinary ones and zeros"""
+    from step_amd import optim
+    sizes = [1.0, 1e-4, 3e-7, 2e-6, 0.0, 1e-5]
+    eps = 1e-4
+    for m, n in ((100, 140), (20, 140), (90, 2700)):
+        g = torch.stack([matrices(m, n, seed=i).div_(matrices(m, n, seed=i).norm()) * s for i, s in enumerate(sizes)]).to(dtype)
+        o = optim.newton_schulz(g, eps=eps)
+        ref = orthogonalised(g, 5, eps)
+        for i, s in enumerate(sizes):
+            if not g[i].any():                                # (fp16 holds nothing of the smallest)
+                assert not o[i].any()
+                continue
+            # 16 bits: half a unit of the smallest number beside the relative rounding, in every element
+            tiny = math.sqrt(m * n) * torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 / float(ref[i].norm())
+            close(o[i], ref[i], tolerance(m, n, dtype) + tiny, (m, n, s))
