@@ -278,7 +278,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const SmallArgs
     if (tid < 64) {                                          // the trace is the squared norm
         double tr = tid < R ? A[tid * S_P + tid] : 0.0;
         for (int o = 1; o < 64; o <<= 1) tr += __shfl_xor(tr, o, 64);
-        if (tid == 0) norm_s = 1.0 / (sqrt(tr) + (double)p.eps);
+        if (tid == 0) norm_s = tr == 0.0 ? 0.0 : 1.0 / (sqrt(tr) + (double)p.eps);      // (a zero matrix stays zero)
     }
     __syncthreads();
     const double inv = norm_s;
@@ -466,8 +466,8 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(const Big p) {
     // (head: 0 of 0 / 0, and where there are NaN or infinities)
     const float head = size > 0.0 ? -((float)__builtin_amdgcn_frexp_exp(size) + __builtin_amdgcn_logf((float)__builtin_amdgcn_frexp_mant(size))) : 0.f;
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) heads(p)[z] = head;
-    // 2^lift SX / (norm + eps) in two factors, for either may be beyond fp32
-    const double scale = (double)SX / over;
+    // 2^lift SX / (norm + eps) in two factors, for either may be beyond fp32; a zero matrix stays zero
+    const double scale = norm == 0.0 ? 0.0 : (double)SX / over;
     const int power = __builtin_amdgcn_frexp_exp(scale) + lift(head, 0);
     const float factor = (float)__builtin_amdgcn_frexp_mant(scale);
 #pragma unroll

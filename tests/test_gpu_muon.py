@@ -402,3 +402,16 @@ def test_a_stack_of_sizes(dtype):
             # 16 bits: half a unit of the smallest number beside the relative rounding, in every element
             tiny = math.sqrt(m * n) * torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 / float(ref[i].norm())
             close(o[i], ref[i], tolerance(m, n, dtype) + tiny, (m, n, s))
+
+
+@pytest.mark.parametrize("m,n", [(30, 90), (120, 100)])
+def test_zero_without_eps(m, n):
+    """a zero matrix stays zero whatever eps is; the smallest numbers do not count as zeros"""
+    from step_amd import optim
+    assert not optim.newton_schulz(torch.zeros(2, m, n, device=D), eps=0.0).any()
+    p = torch.nn.Parameter(torch.ones(m, n, device=D))
+    p.grad = torch.zeros_like(p)
+    optim.Muon([p], eps=0.0, lr=0.1).step()
+    assert torch.equal(p, torch.ones_like(p))
+    g = matrices(m, n) * 1e-36                                # subnormal elements among them: what fp32 holds of them is the input
+    close(optim.newton_schulz(g, eps=0.0), orthogonalised(g, eps=0.0), tolerance(m, n, torch.float32))
