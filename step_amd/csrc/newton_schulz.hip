@@ -20,7 +20,7 @@
 //   contraction.  A and q(A) are symmetric: only the tiles on and over the diagonal are computed.  Bound by the matrix cores where
 //   the products fill the card (4096 x 4096: X's update 355 us, 1.16 PFLOP/s of f16 products, the cores busy in 65 % of the
 //   cycles at the 1.8 GHz that their power leaves; a plain f16 product of 8192^3 reaches 1.02), by the chain of r x r products
-//   otherwise (256 x 19200: 14 of them, 6 us each, of 170).  An element's error is 2^-23 of it, or 2^-39 where it is under 2^-17
+//   otherwise (256 x 19200: 11 of them, 6 us each, of 187).  An element's error is 2^-23 of it, or 2^-39 where it is under 2^-17
 //   (f16's subnormals hold its lo): of the matrix's size, since X is lifted by a power of two as long as |G| is far below eps
 //   and X with it (lift() below).
 #include <vector>
@@ -892,11 +892,11 @@ struct Share {
 // of them on the matrix cores), 1150 and 1180 at 128 x 128, 690 at 128 x 64, 480 at 64 x 64; a tile's beginning and end, half of
 // which two tiles in a CU share; writing the parts of split tiles and joining them.  All five steps in us:
 //                             as chosen   tiles never split   one 128 x 128 a CU only   128 columns only   256 x 128 only
-//   4096 x 4096 fp32               3640                4165                      3711               3640             3730
-//   3 x 4101 x 1030 bf16            655                 678                       680                762              893
-//   256 x 19200 fp32                170                 377                       177                258              371
-//   1024 x 4096 fp32                302                 315                       303                402              502
-//   512 x 512 fp32                  133                 132                       132                194              249
+//   4096 x 4096 fp32                3660                4178                      3787               3652             3792
+//   3 x 4101 x 1030 bf16             637                 638                       668                764              890
+//   256 x 19200 fp32                 185                 497                       192                276              370
+//   1024 x 4096 fp32                 319                 337                       318                401              503
+//   512 x 512 fp32                   132                 132                       131                194              241
 Share share(int v, long long tiles, long long total) {
     Share s{v, (int)tiles, (int)(total / CUS * CUS), (int)(total % CUS), 1};
     return s;
@@ -922,7 +922,8 @@ Share fastest(int v, long long tiles, int nb, int stages) {
 }
 struct Layout {
     size_t part, x, xt, xt2, r[4], slab, total;
-    int sub, R, L, RA, group;
+    int sub, R, L, RA;
+    bool group;                                   // steps are taken together
     Share xxt, sym, update;
 };
 Layout layout_of(int nb, int r, int l) {
@@ -969,11 +970,11 @@ Layout layout(int batch, int m, int n) {
     o.xt2 = take(sub * R * L * 4);
     // Steps taken together: k steps at once are one X X^T and one P X, P = q(A_k) .. q(A_1), with A_i+1 = q(A_i) A_i q(A_i) from
     // products of r x r matrices, of which each further step takes three more: where the two passes over X cost more than those
-    // (256 x 19200: 170 us, 224 step by step; 3 x 4101 x 1030 655 and 933; 400 x 900, taken step by step, 140, and 150 together; 3.8 passes' worth is
-    // where they are even: 1690 x 71 103 both ways, 2500 x 1000 311 and 277 together).
+    // (3 x 4101 x 1030 bf16: 637 us together, 933 step by step; 400 x 900, taken step by step, 139, and 150 together; 3.8 passes' worth is
+    // where they are even: 1690 x 71 111, step by step).  together() says how many.
     const double passes = cycles(o.xxt, step::ceil_div(l, KS)) + cycles(o.update, step::ceil_div(r, KS));
-    o.group = l >= 2 * r && passes > 3.8 * cycles(o.sym, step::ceil_div(r, KS)) ? 3 : 1;
-    for (int i = 0; i < (o.group > 1 ? 4 : 2); ++i) o.r[i] = take(sub * RA * R * 4);
+    o.group = l >= 2 * r && passes > 3.8 * cycles(o.sym, step::ceil_div(r, KS));
+    for (int i = 0; i < (o.group ? 4 : 2); ++i) o.r[i] = take(sub * RA * R * 4);
     // shares of split tiles: fewer than one a CU, of 256 x 128 at most.  A last part of the batch that is smaller is shared out anew.
     const bool any = sub < batch || o.xxt.splits > 1 || o.sym.splits > 1 || o.update.splits > 1;
     o.slab = take(any ? (size_t)CUS * 256 * 128 * 4 : 0);
@@ -1073,13 +1074,21 @@ int product(const Big& p, const Share& s, hipStream_t st) {
         default: return product_of<PROD, 4, T>(p, s, st);
     }
 }
-// An error of A grows by a^2 = 12 in each step of a group for the smallest eigenvalues.  fp32 results off by, together / step by step
-// (fp32 products of the library: the last figure): 10000 x 100 2.5e-6 / 0.7e-6 (1.5e-6), 6000 x 130 2.0e-6 / 0.8e-6 (1.3e-6),
-// 7000 x 160 1.8e-6 / 1.2e-6 (1.6e-6), 256 x 19200 1.5e-6 / 1.2e-6 (4.4e-6), 6000 x 1000 2.3e-6 / 1.6e-6 (2.8e-6): the narrow ones are
-// taken step by step.  Results of 16 bits are rounded far above that.
+// Steps taken together: the first `first` alone, then `most` at a time, where layout() finds that this pays.  An error of A grows by
+// a^2 = 12 in each step of a group for the smallest eigenvalues, so that three at a time are for results of 16 bits, rounded far above
+// it.  fp32 takes the first step, before which the smallest are smallest, by itself and then two at a time.  Its error over that of
+// fp32 products (the library's), the worst of six kinds of matrices (low rank and noise, Gaussian, singular values over a range of 30
+// and of 1000, ...), step by step / one and two / three at a time: 160 x 6000 1.08 / 1.12 / 1.67, 192 x 14000 1.05 / 1.08 / 1.40,
+// 256 x 9000 1.04 / 1.07 / 1.3, 340 x 6000 1.04 / 1.09 / 1.36, 1000 x 3000 0.93 / 1.05 / 0.96, 1400 x 6000 0.92 / 1.08 / 0.96; not
+// taken together: 130 x 6000 1.13 / 1.17 / 1.52, 1400 x 4000 0.94 / 1.40 / 1.32.  Times: 256 x 19200 218 / 183 / 167 us, 1000 x 6000
+// 450 / 368 / 334, 192 x 7000 152 / 136 / 130.
+struct Together {
+    int first, most;
+};
 template <typename T>
-bool together(int r) {
-    return sizeof(T) < 4 || r >= 160;
+Together together(int r, int l) {
+    if (sizeof(T) < 4) return Together{3, 3};
+    return r >= 160 && l >= 4 * r ? Together{1, 2} : Together{1, 1};
 }
 template <typename T>
 int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* base, hipStream_t st) {
@@ -1096,7 +1105,7 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
     p.part = (double*)(base + all.part);
     p.slab = (float*)(base + all.slab);
     p.x = base + all.x;
-    const int group = together<T>(p.r) ? all.group : 1;
+    const Together group = all.group ? together<T>(p.r, p.l) : Together{1, 1};
     char* r[4];
     for (int i = 0; i < 4; ++i) r[i] = base + all.r[i];
     for (int b0 = 0; b0 < it.batch; b0 += all.sub) {
@@ -1131,7 +1140,7 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
             if (rc == STEP_OK) rc = product<POLY, float>(p, o.sym, st);
         };
         for (int s = 0; s < steps && rc == STEP_OK;) {
-            const int g = steps - s < group ? steps - s : group;
+            const int want = s ? group.most : group.first, g = steps - s < want ? steps - s : want;
             char *A = r[0], *P = r[1], *Q = r[1], *W = r[2], *F = r[3];      // F: free
             p.s3 = A;
             p.scale = SA / (SX * SX);

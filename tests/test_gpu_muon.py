@@ -415,3 +415,28 @@ def test_zero_without_eps(m, n):
     assert torch.equal(p, torch.ones_like(p))
     g = matrices(m, n) * 1e-36                                # subnormal elements among them: what fp32 holds of them is the input
     close(optim.newton_schulz(g, eps=0.0), orthogonalised(g, eps=0.0), tolerance(m, n, torch.float32))
+
+
+def kinds(m, n):
+    """low rank and noise, noise alone, singular values over a range of 30 and of 1000"""
+    gen = torch.Generator().manual_seed(m + n)
+    r, l = min(m, n), max(m, n)
+    u, v = (torch.linalg.qr(torch.randn(k, r, generator=gen).to(D).double())[0] for k in (r, l))
+    yield matrices(m, n, seed=m)
+    yield torch.randn(m, n, generator=gen).to(D)
+    for condition in (30.0, 1000.0):
+        x = (u * condition ** -torch.linspace(0, 1, r, device=D, dtype=torch.float64)) @ v.t().contiguous()
+        yield (x if m <= n else x.t()).float().contiguous()
+
+
+@pytest.mark.parametrize("m,n", [(6000, 160), (160, 8000), (7000, 192), (192, 10000), (224, 6000), (256, 9000), (300, 10000), (340, 3000),
+                                 (500, 6000), (1000, 3000), (1400, 3000), (200, 200)])
+def test_as_exact_as_fp32_products_on_all_kinds(m, n):
+    """root 2 times the error of the iteration with torch's own fp32 products at most.  Of an error's three parts - the operands'
+    rounding, the sums' and the results' - the first is 2^-23 for two halves of 11 bits where fp32 has 2^-24, the others are fp32's
+    (root of (4 + 1 + 1) / 3); it is these that the smallest singular values multiply, on both sides alike"""
+    from step_amd import optim
+    for i, g in enumerate(kinds(m, n)):
+        ref = orthogonalised(g)
+        off = [float((t.double() - ref).norm() / ref.norm()) for t in (optim.newton_schulz(g), orthogonalised32(g))]
+        assert off[0] <= math.sqrt(2) * off[1], (i, off)
