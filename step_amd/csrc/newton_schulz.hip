@@ -88,7 +88,7 @@ __device__ __forceinline__ const SmallItem& find(const SmallArgs& p, int z, int&
     local = z - first;
     return p.item[i];
 }
-__device__ __forceinline__ Io shifted(Io io, size_t by, int bytes) {
+__device__ __host__ __forceinline__ Io shifted(Io io, size_t by, int bytes) {
     io.g = (const char*)io.g + by * bytes;
     if (io.out) io.out = (char*)io.out + by * bytes;
     if (io.momentum) io.momentum += by;
@@ -983,55 +983,76 @@ Layout layout(int batch, int m, int n) {
 }
 bool small(int m, int n) { return (m < n ? m : n) <= 64; }
 
+// matrices [from, from + count) of an item
+struct Piece {
+    int item, from, count, first;          // first: number of its first matrix in the group
+    SmallItem s;
+};
 struct Group {
-    int begin, end;                        // items (indices into the list of small ones)
+    std::vector<Piece> pieces;
     int total, max_chunks, max_parts;
     size_t doubles;
 };
-// small items in groups of one launch each; the workspace is used again by every group
-void small_groups(const step_ns_item* items, const std::vector<int>& idx, std::vector<Group>& groups, std::vector<SmallItem>& out,
-                  std::vector<int>& firsts) {
-    for (size_t i = 0; i < idx.size();) {
-        Group g{(int)i, (int)i, 0, 1, 1, 0};
-        int total = 0;
-        size_t end = i;
-        long long parts = 1;
-        while (end < idx.size() && end - i < (size_t)S_ITEMS) {      // (a launch has fewer than 2^31 blocks)
-            const step_ns_item& it = items[idx[end]];
-            const long long mine = step::ceil_div(it.m > it.n ? it.m : it.n, 64), most = mine > parts ? mine : parts;
-            if (end > i && (total + it.batch) * most >= 1LL << 31) break;
-            parts = most;
-            total += items[idx[end++]].batch;
-        }
-        const int share = total < 1024 ? 1024 / total : 1;
-        int first = 0;
-        size_t at = 0;
-        for (; i < end; ++i) {
-            const step_ns_item& it = items[idx[i]];
+// Matrices of a group: 218 MB of workspace (the sums of one chunk and P, 52 KB a matrix), and sixteen times what the CUs hold at a time.
+// A launch has fewer than 2^32 threads: ns_apply_kernel's bound is the first to be met, 256 threads for each part of each matrix.
+constexpr int GROUP_MATRICES = 4096;
+constexpr int GROUP_PARTS = (1 << 24) - 1;
+// small items in groups of one launch of each kernel; the workspace is used again by every group
+std::vector<Group> small_groups(const step_ns_item* items, int count) {
+    std::vector<Group> groups;
+    auto parts_of = [&](int i) { return step::ceil_div(items[i].m > items[i].n ? items[i].m : items[i].n, 64); };
+    auto room = [&](int parts) { return GROUP_PARTS / parts < GROUP_MATRICES ? GROUP_PARTS / parts : GROUP_MATRICES; };
+    // `of`: the matrices that share the card, for the count of chunks (all of a stack, so that its matrices are added up alike)
+    auto add = [&](std::vector<Piece>& pieces, int of) {
+        Group g{};
+        g.max_chunks = g.max_parts = 1;
+        const int share = of < 1024 ? 1024 / of : 1;
+        for (Piece& p : pieces) {
+            const step_ns_item& it = items[p.item];
             const int l = it.m > it.n ? it.m : it.n;
             int chunks = step::ceil_div(l, 16 * GRAM_WAVES);
             if (chunks > share) chunks = share;
             if (chunks > 32) chunks = 32;
-            SmallItem s{};
-            s.m = it.m;
-            s.n = it.n;
-            firsts.push_back(first);
-            s.width = step::round_up(step::ceil_div(l, chunks), 16);
-            s.chunks = step::ceil_div(l, s.width);
-            s.slab = at;
-            at += (size_t)it.batch * s.chunks * 2560;
-            s.p = at;
-            at += (size_t)it.batch * 4096;
-            first += it.batch;
-            if (s.chunks > g.max_chunks) g.max_chunks = s.chunks;
-            if (step::ceil_div(l, 64) > g.max_parts) g.max_parts = step::ceil_div(l, 64);
-            out.push_back(s);
+            p.s.m = it.m;
+            p.s.n = it.n;
+            p.s.width = step::round_up(step::ceil_div(l, chunks), 16);
+            p.s.chunks = step::ceil_div(l, p.s.width);
+            p.s.slab = g.doubles;
+            g.doubles += (size_t)p.count * p.s.chunks * 2560;
+            p.s.p = g.doubles;
+            g.doubles += (size_t)p.count * 4096;
+            p.first = g.total;
+            g.total += p.count;
+            if (p.s.chunks > g.max_chunks) g.max_chunks = p.s.chunks;
+            if (parts_of(p.item) > g.max_parts) g.max_parts = parts_of(p.item);
         }
-        g.end = (int)end;
-        g.total = first;
-        g.doubles = at;
-        groups.push_back(g);
+        g.pieces.swap(pieces);
+        groups.push_back(std::move(g));
+        pieces.clear();
+    };
+    std::vector<Piece> open;
+    int total = 0, parts = 1;
+    for (int i = 0; i < count; ++i) {
+        if (!small(items[i].m, items[i].n)) continue;
+        const int mine = parts_of(i), most = mine > parts ? mine : parts, batch = items[i].batch;
+        if (!open.empty() && ((int)open.size() == S_ITEMS || batch > room(most) - total)) {
+            add(open, total);
+            total = 0;
+            parts = 1;
+        }
+        if (batch > room(mine)) {                            // a stack of several groups, by itself
+            for (int from = 0; from < batch; from += room(mine)) {
+                std::vector<Piece> one{Piece{i, from, batch - from < room(mine) ? batch - from : room(mine), 0, SmallItem{}}};
+                add(one, batch);
+            }
+            continue;
+        }
+        open.push_back(Piece{i, 0, batch, 0, SmallItem{}});
+        total += batch;
+        if (mine > parts) parts = mine;
     }
+    if (!open.empty()) add(open, total);
+    return groups;
 }
 
 int check(const step_ns_item* items, int count) {
@@ -1176,40 +1197,37 @@ int run_big(const step_ns_item& it, const Io& io, int steps, float eps, char* ba
 
 template <typename T>
 int run(const step_ns_item* items, int count, int steps, float eps, float mu, int nesterov, float lr, float decay, void* ws, hipStream_t st) {
-    std::vector<int> idx;
     auto io_of = [&](const step_ns_item& it) {
         return Io{it.g, it.out, it.momentum, it.param, mu, 1.f - lr * decay, lr * it.scale, nesterov};
     };
-    for (int i = 0; i < count; ++i)
-        if (small(items[i].m, items[i].n)) idx.push_back(i);
-    if (!idx.empty()) {
-        std::vector<Group> groups;
-        std::vector<SmallItem> sm;
-        std::vector<int> firsts;
-        small_groups(items, idx, groups, sm, firsts);
+    const std::vector<Group> groups = small_groups(items, count);
+    if (!groups.empty()) {
         constexpr size_t lds = 3 * 64 * S_P * sizeof(double);
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(ns_small_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) {
             step::set_error("step_newton_schulz: hipFuncSetAttribute(%zu): %s", lds, hipGetErrorString(e));
             return STEP_ERR_LAUNCH;
         }
-        for (const Group& g : groups) {
-            SmallArgs a{};
-            const int n = g.end - g.begin;
-            a.steps = steps;
-            a.max_chunks = g.max_chunks;
-            a.max_parts = g.max_parts;
-            a.eps = eps;
-            a.ws = (double*)ws;
-            for (int i = 0; i < S_ITEMS; ++i) a.first[i] = i < n ? firsts[g.begin + i] : 0x7fffffff;
-            for (int i = 0; i < n; ++i) {
-                a.item[i] = sm[g.begin + i];
-                a.item[i].io = io_of(items[idx[g.begin + i]]);
-            }
-            hipLaunchKernelGGL(ns_gram_kernel<T>, dim3((unsigned)g.total * g.max_chunks), dim3(64 * GRAM_WAVES), 0, st, a);
-            hipLaunchKernelGGL(ns_small_kernel, dim3((unsigned)g.total), dim3(SMALL_THREADS), lds, st, a);
-            hipLaunchKernelGGL(ns_apply_kernel<T>, dim3((unsigned)g.total * g.max_parts), dim3(256), 0, st, a);
+    }
+    for (const Group& g : groups) {
+        constexpr size_t lds = 3 * 64 * S_P * sizeof(double);
+        SmallArgs a{};
+        const int n = (int)g.pieces.size();
+        a.steps = steps;
+        a.max_chunks = g.max_chunks;
+        a.max_parts = g.max_parts;
+        a.eps = eps;
+        a.ws = (double*)ws;
+        for (int i = 0; i < S_ITEMS; ++i) a.first[i] = i < n ? g.pieces[i].first : 0x7fffffff;
+        for (int i = 0; i < n; ++i) {
+            const Piece& p = g.pieces[i];
+            const step_ns_item& it = items[p.item];
+            a.item[i] = p.s;
+            a.item[i].io = shifted(io_of(it), (size_t)p.from * it.m * it.n, sizeof(T));
         }
+        hipLaunchKernelGGL(ns_gram_kernel<T>, dim3((unsigned)g.total * g.max_chunks), dim3(64 * GRAM_WAVES), 0, st, a);
+        hipLaunchKernelGGL(ns_small_kernel, dim3((unsigned)g.total), dim3(SMALL_THREADS), lds, st, a);
+        hipLaunchKernelGGL(ns_apply_kernel<T>, dim3((unsigned)g.total * g.max_parts), dim3(256), 0, st, a);
     }
     for (int i = 0; i < count; ++i) {
         if (small(items[i].m, items[i].n)) continue;
@@ -1224,21 +1242,13 @@ int run(const step_ns_item* items, int count, int steps, float eps, float mu, in
 extern "C" size_t step_newton_schulz_ws_bytes(const step_ns_item* items, int count) {
     if (check(items, count) != STEP_OK) return 0;
     try {
-        std::vector<int> idx;
         size_t most = 256;
         for (int i = 0; i < count; ++i) {
-            if (small(items[i].m, items[i].n)) {
-                idx.push_back(i);
-                continue;
-            }
+            if (small(items[i].m, items[i].n)) continue;
             const size_t b = layout(items[i].batch, items[i].m, items[i].n).total;
             if (b > most) most = b;
         }
-        std::vector<Group> groups;
-        std::vector<SmallItem> sm;
-        std::vector<int> firsts;
-        small_groups(items, idx, groups, sm, firsts);
-        for (const Group& g : groups)
+        for (const Group& g : small_groups(items, count))
             if (g.doubles * sizeof(double) > most) most = g.doubles * sizeof(double);
         return most;
     } catch (...) {

@@ -198,3 +198,17 @@ def test_policy_logits_of_a_saturated_softmax():
     (logits * torch.tensor([[1.0, -1.0, 0.5]])).sum().backward()
     assert bool(logits.isfinite().all()) and bool(x.grad.isfinite().all())
     assert torch.equal(logits[0, 0], torch.log(torch.softmax(x, 1))[0, 0])
+
+
+def ns_bytes(*shapes):
+    return _lib.query("step_newton_schulz_ws_bytes", (_lib.NsItem * len(shapes))(*[_lib.NsItem(4096, 4096, None, None, *s, 1.0) for s in shapes]), len(shapes))
+
+
+@pytest.mark.parametrize("shapes", [
+    [(1000000, 4, 4)], [(1 << 24, 2, 2)], [(1 << 20, 64, 64)], [(600, 64, 1 << 21)], [(1, 64, 1 << 21), (512, 8, 8)],
+    [(512, 8, 8), (1, 64, 1 << 21), (5000, 30, 200)], [(300, 20, 40)] * 100, [(4095, 3, 3), (2, 3, 3), (4096, 3, 3), (4097, 3, 3)]])
+def test_the_workspace_of_many_small_matrices_is_bounded(shapes):
+    """they are taken in groups, at most 4096 matrices each, of 6656 fp64 numbers (a chunk's sums, P) and of 31 more chunks of 2560 where
+    fewer than 1024 matrices share the card"""
+    assert 0 < ns_bytes(*shapes) <= 8 * (4096 * 6656 + 1024 * 2560)
+    assert ns_bytes(*shapes) >= 8 * 6656 * min(sum(s[0] for s in shapes), 500)

@@ -440,3 +440,30 @@ def test_as_exact_as_fp32_products_on_all_kinds(m, n):
         ref = orthogonalised(g)
         off = [float((t.double() - ref).norm() / ref.norm()) for t in (optim.newton_schulz(g), orthogonalised32(g))]
         assert off[0] <= math.sqrt(2) * off[1], (i, off)
+
+
+def test_more_small_matrices_than_a_launch_takes():
+    """stacks and lists that are divided: each launch has a matrix of many blocks' work beside a stack, or more matrices than one
+    launch may have blocks of 256 to 1024 threads"""
+    from step_amd import optim
+    g = matrices(1000000, 4, 4, seed=1)
+    o = optim.newton_schulz(g)
+    for at in (slice(0, 5), slice(4090, 4100), slice(999990, None)):
+        close(o[at], orthogonalised(g[at]), tolerance(4, 4, torch.float32))
+    ref = orthogonalised(g)
+    per = (o.double() - ref).norm(dim=(1, 2)) / ref.norm(dim=(1, 2))
+    assert float(per.max()) <= tolerance(4, 4, torch.float32)
+    g = matrices(5000, 33, 70, seed=2)
+    o = optim.newton_schulz(g)
+    close(o, orthogonalised(g), tolerance(33, 70, torch.float32))
+    same = optim.newton_schulz(g[:1].expand(5000, 33, 70))    # one matrix is one result, wherever it lies in a stack
+    assert torch.equal(same, same[:1].expand(5000, 33, 70))
+
+
+def test_a_long_matrix_beside_a_stack():
+    from step_amd import optim
+    long, wide = (torch.randn(*s, generator=torch.Generator(D).manual_seed(i), device=D) for i, s in enumerate([(64, 1 << 21), (1 << 21, 3)]))
+    stack = matrices(512, 8, 8, seed=3)
+    outs = optim.newton_schulz([long, stack, wide])
+    for g, o in zip((long, stack, wide), outs):
+        close(o, orthogonalised(g), tolerance(1, 1, torch.float32), tuple(g.shape))
