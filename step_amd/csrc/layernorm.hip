@@ -228,19 +228,22 @@ __global__ __launch_bounds__(1024) void ln_join_kernel(const float* __restrict__
                                                        void* __restrict__ db, int lines, int cols, int wdtype) {
     __shared__ float sm[32][33];
     const int j = threadIdx.x & 31, k = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + j;
-    float s = 0.f;
-    if (c < 2 * cols)
-        for (int l = k; l < lines; l += 32) s += part[(size_t)l * 2 * cols + c];
-    sm[k][j] = s;
-    __syncthreads();
-    if (k == 0 && c < 2 * cols) {
-        for (int i = 1; i < 32; ++i) s += sm[i][j];
-        if (c < cols) {
-            if (dw) store_as(dw, c, wdtype, s);
-        } else if (db) {
-            store_as(db, c - cols, wdtype, s);
+    for (int c0 = blockIdx.x * 32; c0 < 2 * cols; c0 += gridDim.x * 32) {
+        const int c = c0 + j;
+        float s = 0.f;
+        if (c < 2 * cols)
+            for (int l = k; l < lines; l += 32) s += part[(size_t)l * 2 * cols + c];
+        sm[k][j] = s;
+        __syncthreads();
+        if (k == 0 && c < 2 * cols) {
+            for (int i = 1; i < 32; ++i) s += sm[i][j];
+            if (c < cols) {
+                if (dw) store_as(dw, c, wdtype, s);
+            } else if (db) {
+                store_as(db, c - cols, wdtype, s);
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -313,25 +316,34 @@ __global__ __launch_bounds__(1024) void ln_cols_long_kernel(const T* __restrict_
                                                             long long rows, int cols) {
     __shared__ float sm[16][2][64];
     const int j = threadIdx.x & 63, k = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + j;
-    float s1 = 0.f, s2 = 0.f;
-    if (c < cols)
-        for (long long row = (long long)blockIdx.y * 16 + k; row < rows; row += (long long)gridDim.y * 16) {
-            const float g = (float)dy[(size_t)row * cols + c];
-            s1 += g * (((float)x[(size_t)row * cols + c] - mean[row]) * rstd[row]);
-            s2 += g;
+    for (int c0 = blockIdx.x * 64; c0 < cols; c0 += gridDim.x * 64) {
+        const int c = c0 + j;
+        float s1 = 0.f, s2 = 0.f;
+        if (c < cols)
+            for (long long row = (long long)blockIdx.y * 16 + k; row < rows; row += (long long)gridDim.y * 16) {
+                const float g = (float)dy[(size_t)row * cols + c];
+                s1 += g * (((float)x[(size_t)row * cols + c] - mean[row]) * rstd[row]);
+                s2 += g;
+            }
+        sm[k][0][j] = s1;
+        sm[k][1][j] = s2;
+        __syncthreads();
+        if (k < 2 && c < cols) {
+            float s = 0.f;
+            for (int i = 0; i < 16; ++i) s += sm[i][k][j];
+            part[(size_t)blockIdx.y * 2 * cols + k * cols + c] = s;
         }
-    sm[k][0][j] = s1;
-    sm[k][1][j] = s2;
-    __syncthreads();
-    if (k < 2 && c < cols) {
-        float s = 0.f;
-        for (int i = 0; i < 16; ++i) s += sm[i][k][j];
-        part[(size_t)blockIdx.y * 2 * cols + k * cols + c] = s;
+        __syncthreads();
     }
 }
 
 constexpr int MAX_LINES = 512;
+// blocks over the columns, which go on to further ones: a launch has fewer than 2^32 threads, and rows up to 2^28 columns
+constexpr int MAX_COLUMN_BLOCKS = 1 << 16;
+int column_blocks(long long cols, int per) {
+    const long long blocks = (cols + per - 1) / per;
+    return (int)(blocks < MAX_COLUMN_BLOCKS ? blocks : MAX_COLUMN_BLOCKS);
+}
 
 struct Plan {
     int g, nv, vec;                 // threads per row, packs per thread, elements of a pack; g 0: too long for the registers of 1024 threads
@@ -456,7 +468,7 @@ extern "C" int step_layernorm_bwd(const void* dy, const void* x, const void* w, 
                 hipLaunchKernelGGL(ln_bwd_long_kernel<T>, dim3((unsigned)blocks), dim3(1024), 0, st, (const T*)dy, (const T*)x,
                                    w, mean, rstd, (T*)dx, rows, cols, wdtype);
             if (sums)
-                hipLaunchKernelGGL(ln_cols_long_kernel<T>, dim3(step::ceil_div(cols, 64), lines), dim3(1024), 0, st,
+                hipLaunchKernelGGL(ln_cols_long_kernel<T>, dim3(column_blocks(cols, 64), lines), dim3(1024), 0, st,
                                    (const T*)dy, (const T*)x, mean, rstd, part, rows, cols);
             return 0;
         }
@@ -469,6 +481,6 @@ extern "C" int step_layernorm_bwd(const void* dy, const void* x, const void* w, 
         return 0;
     });
     if (sums)
-        hipLaunchKernelGGL(ln_join_kernel, dim3((2 * (unsigned)cols + 31) / 32), dim3(1024), 0, st, part, dw, db, lines, cols, wdtype);
+        hipLaunchKernelGGL(ln_join_kernel, dim3(column_blocks(2LL * cols, 32)), dim3(1024), 0, st, part, dw, db, lines, cols, wdtype);
     return step::check_launch("step_layernorm_bwd");
 }

@@ -227,3 +227,16 @@ def test_hybrid_classifier_with_a_layer_norm_head():
     m.train()
     torch.nn.functional.cross_entropy(m(xa[:1], xg[:1]), torch.tensor([2], device=D)).backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+@pytest.mark.parametrize("rows,cols,dtype", [(3, 1 << 26, torch.float32), (1, (1 << 28) - 3, torch.bfloat16), (2, (1 << 27) + 1, torch.float16)])
+def test_the_longest_rows(rows, cols, dtype, monkeypatch):
+    """up to the 2^28 columns that layer_norm takes: the weights' gradients are joined by fewer blocks than there are columns.  A
+    thread's chain of additions is cols / 1024 long here, all in one direction at worst"""
+    import sys
+    monkeypatch.setattr(sys.modules[__name__], "K", K + cols / 1024)
+    g = torch.Generator(D).manual_seed(cols)
+    x, dy = (torch.randn(rows, cols, generator=g, device=D).to(dtype) for _ in range(2))
+    w, b = ((1 + 0.3 * torch.randn(cols, generator=g, device=D)).to(dtype) for _ in range(2))
+    check(x, w, b, dy)
+    torch.cuda.empty_cache()
