@@ -44,6 +44,9 @@ enum step_dtype {
 int step_abi_version(void);
 const char* step_last_error(void);
 
+/* the capture that `stream` is in, a number of its own; 0 where it is in none */
+unsigned long long step_capture_id(void* stream);
+
 /* ---------------------------------------------------------------- BatchNorm --------
  * group layout `bn_mode`:
  *   0: group = c        nn.BatchNorm2d over (N,T,V)            classifier.py:154,163,180
@@ -533,9 +536,10 @@ int step_layernorm_bwd(const void* dy, const void* x, const void* w, const float
  * fp32, mask bytes (nullable: every row is live), one per row.  loss[1], stats[3] = {policy part, KL, share of clipped rows},
  * logp[rows] (0 in masked rows) fp32; dlogits (nullable) like logits.  A masked row is not read.  An action outside
  * [0, classes) of a live row makes the loss and the row's gradient NaN; nothing is read there.
- * With `upstream` (a device scalar) only dlogits is written, times *upstream; skip_one: nothing is done where *upstream is
- * exactly 1 (the caller's dlogits already holds that gradient), and ws is the one that the call without `upstream` left (it
- * holds the number of live rows, and long rows' sums).  ws: step_policy_loss_ws_bytes(rows, classes).           */
+ * With `upstream` (a device scalar) only dlogits is written, times *upstream.  skip_one: ws is the one that the call without
+ * `upstream` left (it holds the number of live rows, and long rows' sums), and nothing is done where *upstream is exactly 1
+ * (the caller's dlogits already holds that gradient); without it the call takes them again and depends on no other.
+ * ws: step_policy_loss_ws_bytes(rows, classes).                                                              */
 size_t step_policy_loss_ws_bytes(long long rows, int classes);
 int step_policy_loss(const void* logits, const long long* actions, const float* old_logp, const float* advantages,
                      const float* ref_logp, const unsigned char* mask, double clip_low, double clip_high, double beta,

@@ -108,6 +108,7 @@ SIGNATURES = {
     "step_bn_rows_bwd_apply": (I, [P, P, P, P, P, P, P, I, I, P]),
     "step_softmax_fwd": (I, [P, P, I, I, P]),
     "step_softmax_bwd": (I, [P, P, P, I, I, P]),
+    "step_capture_id": (ctypes.c_ulonglong, [P]),
     "step_layernorm_fwd": (I, [P, P, P, P, P, P, LL, I, I, I, F, P]),
     "step_layernorm_bwd_ws_bytes": (Z, [LL, I]),
     "step_layernorm_bwd": (I, [P, P, P, P, P, P, P, P, LL, I, I, I, P, Z, P]),
@@ -146,6 +147,11 @@ def load():
 def stream(device=None):
     index = device.index if device is not None and device.index is not None else torch.cuda.current_device()
     return torch._C._cuda_getCurrentRawStream(index)     # (no Stream object: 0.3 us a launch instead of 2 to 9)
+
+
+def capture(device):
+    """the graph capture that the device's current stream is in (None: none), which two calls can be compared by"""
+    return query("step_capture_id", stream(device)) if torch.cuda.is_current_stream_capturing() else None
 
 
 def call(name, *args):

@@ -27,3 +27,12 @@ const char* last_error() { return g_err; }
 
 extern "C" int step_abi_version(void) { return STEP_ABI_VERSION; }
 extern "C" const char* step_last_error(void) { return step::last_error(); }
+extern "C" unsigned long long step_capture_id(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();             // (the next launch's check is not to see it)
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? id : 0;
+}

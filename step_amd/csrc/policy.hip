@@ -34,7 +34,7 @@ struct Args {
     const double* count;           // device: number of live rows (NULL: all of them)
     double* part;                  // [blocks][3]
     const float* upstream;         // NULL: the loss itself; else only dlogits, times *upstream
-    int skip_one;                  // with upstream: nothing to do where it is exactly 1
+    int skip_one;                  // with upstream: nothing to do where it is exactly 1, and count and a long row's sums are there
     long long rows;
     int classes;
     double clip_low, clip_high, beta;   // a clipped ratio's 1.2 in fp32 is off by 4e-8, the same way in every row
@@ -461,7 +461,7 @@ void launch(const Plan& pl, int blocks, const Args& a, hipStream_t st) {
 template <typename T>
 void launch_parts(int parts, int span, int blocks, const Args& a, Row* soft, hipStream_t st) {
     constexpr int N = 16 / (int)sizeof(T);
-    if (!a.upstream) hipLaunchKernelGGL((policy_parts_kernel<T, N, false>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
+    if (!a.skip_one) hipLaunchKernelGGL((policy_parts_kernel<T, N, false>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
     hipLaunchKernelGGL((policy_parts_kernel<T, N, true>), dim3(blocks), dim3(256), 0, st, a, soft, parts, span);
 }
 
@@ -499,7 +499,8 @@ extern "C" int step_policy_loss(const void* logits, const long long* actions, co
         parts = parts_of(classes, pl.vec, span);
         blocks = rows * parts < MAX_BLOCKS ? (int)(rows * parts) : MAX_BLOCKS;
     }
-    if (mask && !upstream) hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(1024), 0, st, mask, count, rows);
+    if (!upstream) skip_one = 0;
+    if (mask && !skip_one) hipLaunchKernelGGL(policy_count_kernel, dim3(1), dim3(1024), 0, st, mask, count, rows);
     const Args a{logits, actions, old_logp, advantages, ref_logp, mask, dlogits, logp, mask ? count : nullptr, part,
                  upstream, skip_one, rows, classes, clip_low, clip_high, beta};
     auto go = [&](auto t) {

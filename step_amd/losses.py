@@ -67,10 +67,12 @@ def vae_loss(x_in, x_out, mean, lsig, beta=1.):
 class _PolicyLossFn(torch.autograd.Function):
     """The forward leaves the gradient for an upstream gradient of 1 behind (value and gradient take one pass over the
     logits); the backward hands it out, or computes it again from the logits where the upstream gradient is not 1 - on
-    the device, with one rounding - or where a retained graph asks a second time, or a captured backward without its forward."""
+    the device, with one rounding - or where a retained graph asks a second time.  A graph that holds the backward without its
+    forward is replayed when the forward's memory may long be something else's: there it is computed anew from the caller's tensors,
+    and where one of them had to be copied, whose copy is not the caller's to keep, refused."""
 
     @staticmethod
-    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, beta):
+    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, clip_low, clip_high, beta, copied):
         classes = logits.shape[-1]
         rows = logits.numel() // classes
         z = logits.contiguous()
@@ -90,7 +92,8 @@ class _PolicyLossFn(torch.autograd.Function):
                       loss, stats, logp, grad, rows, classes, _lib.DTYPES[z.dtype], ws, nb)
         if need:
             ctx.save_for_backward(z, actions, old_logp, advantages, ref_logp, mask)
-            ctx.grad, ctx.ws, ctx.captured = grad, ws, z.is_cuda and torch.cuda.is_current_stream_capturing()
+            ctx.grad, ctx.ws, ctx.capture = grad, ws, _lib.capture(z.device)
+            ctx.copied = copied or not logits.is_contiguous()
         return loss, logp, stats
 
     @staticmethod
@@ -98,15 +101,19 @@ class _PolicyLossFn(torch.autograd.Function):
     def backward(ctx, g, _logp, _stats):
         z, actions, old_logp, advantages, ref_logp, mask = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
-        # a graph of the backward alone keeps no hold on the forward's memory, and is replayed without it
-        first = grad is not None and (ctx.captured or not torch.cuda.is_current_stream_capturing())
+        capture = _lib.capture(z.device)
+        first = grad is not None and capture == ctx.capture
+        ws = ctx.ws
         if not first:
-            grad = torch.empty_like(z)
+            if ctx.copied and capture is not None and ctx.capture is None:
+                raise _lib.StepHipError("policy_loss: a backward captured without its forward reads the forward's arguments at every "
+                                        "replay: contiguous logits, int64 actions, fp32 and bool of one value a row wanted")
+            grad, ws = torch.empty_like(z), torch.empty_like(ws)
         rows = z.numel() // z.shape[-1]
         if rows:
             _lib.call("step_policy_loss", z, actions, old_logp, advantages, ref_logp, mask, *ctx.config, g.contiguous(),
-                      int(first), None, None, None, grad, rows, z.shape[-1], _lib.DTYPES[z.dtype], ctx.ws, ctx.ws.numel())
-        return (grad,) + (None,) * 8
+                      int(first), None, None, None, grad, rows, z.shape[-1], _lib.DTYPES[z.dtype], ws, ws.numel())
+        return (grad,) + (None,) * 9
 
 
 def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None, clip=0.2, beta=0.0):
@@ -122,7 +129,9 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
     (0 where the mask leaves nothing); ``clip`` is low = high or the pair (low, high).  The loss is differentiable in the
     logits alone.  logp (the rows' log probabilities, 0 where masked) and stats = [policy part, KL, share of clipped rows] are
     fp32 and carry no gradient.  An action outside [0, classes) in a live row makes the loss NaN.  The gradient (of the logits'
-    type, rounded once) is made in the forward already and takes the logits' size in memory until the backward."""
+    type, rounded once) is made in the forward already and takes the logits' size in memory until the backward.  A backward
+    captured into a graph without its forward reads logits, actions and the rows' values at each replay, as they are then: it
+    takes contiguous logits, int64 actions, fp32 and bool of the shape logits.shape[:-1] alone, which stay the caller's."""
     if not isinstance(logits, torch.Tensor) or logits.dim() < 1 or logits.shape[-1] < 1:
         raise _lib.StepHipError("policy_loss: logits (..., classes) wanted")
     if logits.dtype not in _lib.DTYPES:
@@ -135,8 +144,10 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
         raise _lib.StepHipError("policy_loss: clip (%r, %r): 0 <= low <= 1 and high >= 0 wanted" % (low, high))
     lead = logits.shape[:-1]
     where = logits.get_device()
+    copied = False
 
     def per_row(t, name, kinds, to):
+        nonlocal copied
         if not isinstance(t, torch.Tensor) or t.dtype not in kinds:
             raise _lib.StepHipError("policy_loss: %s: a tensor of %s wanted, got %s" % (
                 name, " / ".join(str(k)[6:] for k in kinds), getattr(t, "dtype", type(t).__name__)))
@@ -145,7 +156,9 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
         if t.dtype is to and t.shape == lead and not t.requires_grad and t.is_contiguous():
             return t
         try:
-            return t.detach().to(to).expand(lead).contiguous()
+            r = t.detach().to(to).expand(lead).contiguous()
+            copied = copied or r.data_ptr() != t.data_ptr()
+            return r
         except RuntimeError:
             raise _lib.StepHipError("policy_loss: %s %s does not fit logits %s" % (name, tuple(t.shape), tuple(logits.shape))) from None
 
@@ -157,4 +170,4 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, mask=None,
     mask = per_row(mask, "mask", (torch.bool,), torch.bool) if mask is not None else None
     if not logits.is_cuda:
         raise _lib.StepHipError("step_amd kernels need tensors on the GPU (got device %s); there is no CPU path" % logits.device)
-    return _PolicyLossFn.apply(logits, actions, old_logp, advantages, ref_logp, mask, low, high, beta)
+    return _PolicyLossFn.apply(logits, actions, old_logp, advantages, ref_logp, mask, low, high, beta, copied)

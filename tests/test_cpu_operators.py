@@ -212,3 +212,21 @@ def test_the_workspace_of_many_small_matrices_is_bounded(shapes):
     fewer than 1024 matrices share the card"""
     assert 0 < ns_bytes(*shapes) <= 8 * (4096 * 6656 + 1024 * 2560)
     assert ns_bytes(*shapes) >= 8 * 6656 * min(sum(s[0] for s in shapes), 500)
+
+
+def test_a_captured_backward_of_copies_is_refused(monkeypatch):
+    """on the host, before any launch: the copies that the eager forward made are not the caller's to keep until a replay"""
+    from types import SimpleNamespace
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(_lib, "capture", lambda device: 7)
+    z = torch.zeros(4, 5)
+    for copied, capture, refused in ((True, None, True), (False, None, False), (True, 3, False), (True, 7, False)):
+        ctx = SimpleNamespace(saved_tensors=(z,) * 6, grad=torch.zeros(4, 5), ws=torch.zeros(8, dtype=torch.uint8), capture=capture, copied=copied,
+                              config=(0.2, 0.2, 0.0))
+        what = "captured without its forward" if refused else "no CPU path"      # (what follows is the launch, which takes no CPU tensors)
+        with pytest.raises(StepHipError, match=what):
+            losses._PolicyLossFn.backward(ctx, torch.ones(()), None, None)
+
+
+def test_no_capture_without_a_gpu():
+    assert _lib.query("step_capture_id", None) == 0

@@ -290,3 +290,114 @@ def test_a_captured_backward_without_its_forward(monkeypatch):
     held = again.grad_fn.grad.data_ptr()
     (want,) = torch.autograd.grad(again, leaf)
     assert want.data_ptr() == held and torch.equal(captured, want)
+
+
+@pytest.mark.parametrize("classes", [300, 140001])
+@pytest.mark.parametrize("masked", [True, False])
+def test_a_graph_of_the_backward_alone(classes, masked):
+    """the forward ran eagerly and is gone, its memory taken for something else, when the graph is replayed: each replay is the gradient
+    of the caller's tensors as they are then"""
+    from step_amd import losses
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        z, a, old, adv, ref, mask = inputs((90,), classes, torch.bfloat16)
+        mask = mask if masked else None
+        leaf, up = z.requires_grad_(True), torch.ones((), device=D)
+        loss = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            (grad,) = torch.autograd.grad(loss, leaf, up)
+        del loss
+        torch.cuda.synchronize()
+        taken = [torch.full((n,), float("nan"), device=D) for n in [64] * 50 + [1 << 14] * 50 + [1 << 22] * 8]   # what the forward gave back
+        for k, scale in enumerate((1.0, 2.0, 1.0, 0.5)):
+            fresh = inputs((90,), classes, torch.bfloat16, seed=10 + k)
+            with torch.no_grad():
+                for t, f in zip((leaf, a, old, adv, ref, mask), fresh):
+                    if t is not None:
+                        t.copy_(f)
+                up.fill_(scale)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            again = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+            (want,) = torch.autograd.grad(again, leaf, up)
+            assert torch.equal(grad, want), (k, scale)
+            torch.cuda.synchronize()
+        assert all(bool(t.isnan().all()) for t in taken)
+
+
+def test_a_graph_of_the_backward_alone_takes_no_copies():
+    from step_amd import losses
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        z, a, old, adv, some, _ = inputs((40,), 50, torch.float32)
+        leaf = z.requires_grad_(True)
+        for args in ((a.int(), old, adv), (a, old.double(), adv), (a, old, adv[:1])):
+            loss = losses.policy_loss(leaf, *args)[0]
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                with pytest.raises(losses._lib.StepHipError, match="captured without its forward"):
+                    torch.autograd.grad(loss, leaf, retain_graph=True)
+                some.add_(1.0)                                # (so that the graph holds something)
+            side.synchronize()
+            torch.autograd.grad(loss, leaf)                   # eagerly it has no such needs
+
+
+def test_forward_and_backward_in_two_graphs():
+    """the backward's graph replayed more often than the forward's, with other upstream gradients"""
+    from step_amd import losses
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        z, a, old, adv, ref, mask = inputs((70,), 700, torch.float32)
+        a = a.int()                                           # a copy is made, in the forward's graph
+        leaf, up = z.requires_grad_(True), torch.ones((), device=D)
+        losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)
+        side.synchronize()
+        first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first, stream=side):
+            loss = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+        with torch.cuda.graph(second, stream=side, pool=first.pool()):
+            (grad,) = torch.autograd.grad(loss, leaf, up)
+        for seed, scales in ((5, (1.0, 2.0, 1.0)), (6, (3.0, 1.0)), (7, (1.0,))):
+            with torch.no_grad():
+                for t, f in zip((leaf, a, old, adv, ref, mask), inputs((70,), 700, torch.float32, seed=seed)):
+                    t.copy_(f)
+            first.replay()
+            for scale in scales:
+                up.fill_(scale)
+                second.replay()
+                torch.cuda.synchronize()
+                again = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+                (want,) = torch.autograd.grad(again, leaf, up)
+                assert torch.equal(loss, again) and torch.equal(grad, want), (seed, scale)
+                grad.zero_()                                  # the caller's to change
+                torch.cuda.synchronize()
+
+
+def test_an_eager_backward_of_a_captured_forward():
+    """its gradient is not the graph's memory, which the next replay writes again"""
+    from step_amd import losses
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        z, a, old, adv, ref, mask = inputs((70,), 700, torch.float32)
+        leaf = z.requires_grad_(True)
+        losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            loss = losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0]
+        graph.replay()
+        (grad,) = torch.autograd.grad(loss, leaf)
+        (want,) = torch.autograd.grad(losses.policy_loss(leaf, a, old, adv, ref, mask, beta=0.05)[0], leaf)
+        assert torch.equal(grad, want)
+        adv.neg_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
