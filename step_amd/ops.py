@@ -850,7 +850,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     x float32, bfloat16 or float16; weight and bias (cols,) of x's type or float32, either may be None.  Statistics and
     gradient sums are fp32, every result is rounded once.  Needs no statistics of the batch: a row's result is the same
-    in any batch, on any number of ranks and for a single row."""
+    in any batch, on any number of ranks and for a single row.  The backward reads x, weight and the statistics that the forward saved:
+    a graph that captures it without its forward needs y's autograd graph kept (retain_graph) as long as it is replayed."""
     shape = x.shape
     if not shape or shape[-1] < 1:
         raise _lib.StepHipError("layer_norm: x %s has no last axis to normalise" % (tuple(shape),))
