@@ -50,7 +50,15 @@ struct Row {
     float m;
     double s;
 };
-__device__ __forceinline__ float exp_of(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * L2E); }
+// e^(x - m) scale, an element of the gradient.  fp32: the product with log2 e is rounded at its own size, 2^-19 for a probability of
+// e^-23, and what that is off by, d - y ln 2, is put right in the first order.  16 bits, whose rounding is far above that, do without.
+template <typename T>
+__device__ __forceinline__ float exp_scaled(T x, float m, float scale) {
+    if constexpr (sizeof(T) < 4) return __builtin_amdgcn_exp2f(((float)x - m) * L2E) * scale;
+    const float d = fmaxf(x - m, -1000.f), y = d * L2E;      // (no -inf + inf; a row with a NaN has a NaN as its scale)
+    const float g = __builtin_amdgcn_exp2f(y) * scale;
+    return __builtin_fmaf(g, __builtin_fmaf(y, -LN2_HI, d), g);
+}
 // for the sum, whose logarithm the loss hangs on: the product with log2 e to 48 bits, rounded once (fp32's log2 e alone is off by
 // 1.3e-8, the same way for all elements: log probabilities 3.5e-8 too low on average over 613 classes)
 __device__ __forceinline__ float exp_for_sum(float x, float m) {
@@ -170,7 +178,7 @@ template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> gradient_of(const Pack<T, N>& z, float m, float scale) {
     Pack<T, N> g;
 #pragma unroll
-    for (int e = 0; e < N; ++e) g.v[e] = (T)(exp_of((float)z.v[e], m) * scale);       // the gradient's only rounding
+    for (int e = 0; e < N; ++e) g.v[e] = (T)exp_scaled(z.v[e], m, scale);       // the gradient's only rounding to fewer bits
     return g;
 }
 // adds N elements to a thread's maximum and sum: their largest first, so that nothing overflows
@@ -288,7 +296,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G, G == 1024 ? 4 : 3) void policy_k
 #pragma unroll
         for (int i = 0; i < NV; ++i) own.store(g, i, gradient_of<T, N>(v[i], w.m, scale));
         // the thread that wrote the action's element writes it once more
-        if (valid && lane == action / N % G) g[action] = (T)(exp_of((float)z[action], w.m) * scale + coef);
+        if (valid && lane == action / N % G) g[action] = (T)(exp_scaled(z[action], w.m, scale) + coef);
     }
     if (!p.upstream) block_sums<BLOCK>(p.part, sums);
 }
@@ -361,7 +369,7 @@ __global__ __launch_bounds__(256) void policy_parts_kernel(const Args p, Row* so
             for (int i = 0; i < PART_PACKS; ++i) own.store(g + c0, i, gradient_of<T, N>(v[i], f.m, scale));
             // the thread that wrote the action's element writes it once more
             const long long at = a64 - c0;
-            if (valid && at >= 0 && at < own.cols && tid == (int)at / N % 256) g[a64] = (T)(exp_of((float)z[a64], f.m) * scale + coef);
+            if (valid && at >= 0 && at < own.cols && tid == (int)at / N % 256) g[a64] = (T)(exp_scaled(z[a64], f.m, scale) + coef);
         }
     }
     if (GRAD && !p.upstream) block_sums<256>(p.part, sums);

@@ -401,3 +401,24 @@ def test_an_eager_backward_of_a_captured_forward():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(grad, want)
+
+
+@pytest.mark.parametrize("classes", [5, 300, 4000, 20000, 70003, 140001])
+def test_small_probabilities_of_fp32_rows(classes):
+    """gradients of classes far below the maximum, which is 0 so that no difference is rounded.  In units of u: the exponential 2, the
+    exponent's correction 2 (an fp32 ln 2 times at most 46), roundings of its two products, the scale, its sum and division 6, the
+    sum's smallest terms (127 a thread at most, under 8e-10 each) 2: 12 u of each element"""
+    from step_amd import losses
+    g = torch.Generator().manual_seed(classes)
+    rows = max(3, 60000 // classes)
+    z = (-32 + 11 * torch.rand(rows, classes, generator=g)).to(D)
+    a = torch.randint(0, classes, (rows,), generator=g).to(D)
+    z[torch.arange(rows), a] = 0
+    old, adv = (0.05 * torch.randn(rows, generator=g)).to(D), torch.randn(rows, generator=g).to(D)
+    leaf = z.requires_grad_(True)
+    (grad,) = torch.autograd.grad(losses.policy_loss(leaf, a, old, adv)[0], leaf)
+    _, _, _, ref, _, _ = reference(z, a, old, adv, None, None, 0.2, 0.2, 0.0)
+    others = torch.ones_like(z, dtype=torch.bool)
+    others[torch.arange(rows), a] = False
+    off = (grad.double() - ref).abs()[others] / ref.abs()[others]
+    assert float(off[ref[others] != 0].max()) <= 12 * U, float(off[ref[others] != 0].max()) / U
