@@ -422,3 +422,44 @@ def test_small_probabilities_of_fp32_rows(classes):
     others[torch.arange(rows), a] = False
     off = (grad.double() - ref).abs()[others] / ref.abs()[others]
     assert float(off[ref[others] != 0].max()) <= 12 * U, float(off[ref[others] != 0].max()) / U
+
+
+@pytest.mark.parametrize("rows,classes,dtype", [(20000, 7, torch.float32), (20000, 613, torch.float32), (20000, 613, torch.bfloat16), (20000, 4000, torch.float32),
+                                                (8000, 20000, torch.float32), (8000, 50257, torch.float32), (4000, 100003, torch.float32),
+                                                (4000, 140001, torch.bfloat16)])
+def test_log_probabilities_have_no_bias(rows, classes, dtype):
+    """the mean of the signed errors.  A row's error has no sign of its own: the result's rounding, uniform within 2^-21 for a log
+    probability under 16 (a standard deviation of 2.8e-7), and the sum's, under 2 u; over the rows 3e-7 / root of rows, of which
+    four, and 2e-9 for what the exponential itself leans to"""
+    from step_amd import losses
+    g = torch.Generator(D).manual_seed(classes)
+    z = (2 * torch.randn(rows, classes, device=D, generator=g)).to(dtype)
+    a = torch.randint(0, classes, (rows,), device=D, generator=g)
+    zero = torch.zeros(rows, device=D)
+    _, logp, _ = losses.policy_loss(z, a, zero, zero)
+    bias = []
+    for k in range(0, rows, 1000):
+        part = z[k:k + 1000].double()
+        bias.append((logp[k:k + 1000].double() - (part.gather(1, a[k:k + 1000, None])[:, 0] - torch.logsumexp(part, 1))).sum())
+    bias = float(sum(bias)) / rows
+    assert abs(bias) <= 4 * 3e-7 / rows ** 0.5 + 2e-9, bias
+
+
+def test_a_loss_whose_terms_cancel():
+    """65536 rows whose terms cancel to 1e-4 of their size: the loss is good to 1e-5, that is to 1e-9 of the terms (a row's ratio is off
+    by u at random, of the mean over the rows four standard deviations are 9.3e-10, and its one rounding is 6e-12)"""
+    from step_amd import losses
+    g = torch.Generator(D).manual_seed(1)
+    rows, classes = 65536, 372
+    z = 2 * torch.randn(rows, classes, device=D, generator=g)
+    a = torch.randint(0, classes, (rows,), device=D, generator=g)
+    lp = torch.log_softmax(z.double(), 1).gather(1, a[:, None])[:, 0]
+    old = (lp + 0.05 * torch.randn(rows, device=D, generator=g)).float()
+    adv = torch.randn(rows, device=D, generator=g)
+    rho = torch.exp(lp - old.double())
+    adv = adv - (rho.clamp(0.8, 1.2) * adv.double()).mean().float() + 1e-4     # (ratios within the clipping: terms rho A)
+    loss, _, stats = losses.policy_loss(z, a, old, adv)
+    terms = torch.minimum(rho * adv.double(), rho.clamp(0.8, 1.2) * adv.double())
+    want, size = -float(terms.mean()), float(terms.square().mean().sqrt())
+    assert abs(want) <= 1e-3 * size
+    assert abs(float(loss) - want) <= 4 * U / rows ** 0.5 * size + U * abs(want), (float(loss), want)
