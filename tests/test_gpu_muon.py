@@ -467,3 +467,23 @@ def test_a_long_matrix_beside_a_stack():
     outs = optim.newton_schulz([long, stack, wide])
     for g, o in zip((long, stack, wide), outs):
         close(o, orthogonalised(g), tolerance(1, 1, torch.float32), tuple(g.shape))
+
+
+@pytest.mark.parametrize("shape,dtype", [((3, 2101, 530), torch.bfloat16), ((256, 9600), torch.float32), ((1781, 1810), torch.float16), ((70, 9, 33), torch.float32)])
+def test_the_same_bits_on_any_stream_and_memory(shape, dtype):
+    """split tiles, steps taken together, stacks: called again beside other work, in memory that held something else"""
+    from step_amd import optim
+    g = matrices(*shape, dtype=dtype)
+    want = optim.newton_schulz(g)
+    side = torch.cuda.Stream()
+    for k in range(6):
+        junk = torch.full((1 << 26,), float("nan"), device=D)
+        del junk
+        stream = side if k % 2 else torch.cuda.current_stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            got = optim.newton_schulz(g)
+        if k % 2:
+            optim.newton_schulz(g)                            # on the other stream meanwhile
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), k
