@@ -659,7 +659,7 @@ __device__ __forceinline__ void lds_frag(const float* p, float (&out)[CT]) {
 }
 
 // acc += c * (src rotated right by R lanes inside its row of 16) as ONE instruction.  hipcc leaves
-// __builtin_amdgcn_mov_dpp + fmaf as v_mov_b32_dpp + (SLP-packed) v_pk_fma_f32 - twice the VALU work, and every VALU
+// __builtin_amdgcn_mov_dpp + fmaf as v_mov_b32_dpp + an fma (a packed one where it may) - twice the VALU work, and every VALU
 // cycle of this wave adds to its fp32 MFMA time.  `first` pads the SALU-writes-EXEC -> DPP hazard (5 wait states)
 // that the compiler does not see through an asm statement; the DPP source is an MFMA result that is dozens of MFMAs
 // old by the time these run (the callers fence with sched_barrier).

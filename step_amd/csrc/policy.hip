@@ -7,7 +7,7 @@
 //
 // Memory-bound: the least is one read of the live rows' logits and one write of the gradient.  A row stays in the
 // registers of the G threads that share it between its softmax sums and its gradient (up to 128 K classes in 16 bits,
-// 64 K in fp32; 8192 x 32000 bf16 with 0.7 of the rows live: 198 us, 4.5 TB/s; 16384 x 8000 fp32: 206 us, 5.1 TB/s); longer
+// 64 K in fp32; 8192 x 32000 bf16 with 0.8 of the rows live: 200 us, 4.7 TB/s; 16384 x 8000 fp32: 209 us, 5.0 TB/s); longer
 // rows are read twice.  The number of live rows, which every row's gradient is divided by, is
 // counted by a launch before.  A row's few scalars are taken in fp64: its ratio may lie next to the border of the
 // clipping.  Per-block fp64 sums are added in block order by the last launch: the same bits every time, no atomics.
