@@ -430,7 +430,7 @@ def test_small_probabilities_of_fp32_rows(classes):
 def test_log_probabilities_have_no_bias(rows, classes, dtype):
     """the mean of the signed errors.  A row's error has no sign of its own: the result's rounding, uniform within 2^-21 for a log
     probability under 16 (a standard deviation of 2.8e-7), and the sum's, under 2 u; over the rows 3e-7 / root of rows, of which
-    four, and 2e-9 for what the exponential itself leans to"""
+    four, and 2e-9.  (The exponential of the hardware leans by up to 1e-8, which leaves two of the four.)"""
     from step_amd import losses
     g = torch.Generator(D).manual_seed(classes)
     z = (2 * torch.randn(rows, classes, device=D, generator=g)).to(dtype)
